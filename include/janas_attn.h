@@ -364,6 +364,185 @@ int janas_attn_cache_copy(const struct janas_attn_cache *c, uint32_t n_pos,
                           uint32_t rows, void *k, void *v, float *ks,
                           float *vs, int out, void *stream);
 
+/* ===== Part 4: a paged cache =========================================
+   Keys and values of many sequences in one pool of pages, for programs
+   that serve sequences of unlike and growing lengths: position p of a
+   sequence is row p mod page of the page its block table names for block
+   p / page. Lengths, tables and the free pages live on the device and are
+   read there, so a serving step (janas_attn_pages_plan, _write, _run) makes
+   the same calls whatever the lengths are and can be captured into a graph
+   once. No counterpart in the reference, whose sequences each own a cache.
+   All take a stream (NULL: the default stream), are asynchronous, allocate
+   nothing, and return 0 or a negative JANAS_ATTN_E* code. Arrays are device
+   memory and may not overlap unless it is said. */
+
+/* n_new of a sequence that is done: its pages go back to the free ones */
+#define JANAS_ATTN_RELEASE 0xFFFFFFFFu
+/* a slot or a selected block that is none */
+#define JANAS_ATTN_NONE 0xFFFFFFFFu
+
+/* A pool and its sequences. janas_attn_pages_plan reads the second half
+   alone (k, v may be NULL there). */
+struct janas_attn_pages {
+    void *k, *v;          /* n_pages x n_kv x page x head_dim of kv_type */
+    float *ks, *vs;       /* n_pages x n_kv x page (int8 / int16) */
+    uint16_t *bounds;     /* n_pages x n_kv x 2 x head_dim halves: the smallest
+                             and the largest number of the page's keys in each
+                             dimension (janas_attn_pages_bounds), or NULL */
+    uint32_t n_kv, head_dim;
+    int kv_type;          /* enum janas_attn_kv */
+    uint32_t page;        /* positions a page: 16, 32, 64, 128 or 256 */
+    uint32_t n_pages;     /* n_pages x page below 2^31 */
+    uint32_t n_seqs;      /* up to 65535 */
+    uint32_t max_pages;   /* blocks a table row holds; x page below 2^31 */
+    uint32_t *table;      /* n_seqs x max_pages: the page of each block */
+    uint32_t *len;        /* n_seqs: positions in the cache */
+    uint32_t *free_pages; /* n_pages: the free pages are the first n_free, a
+                             stack (NULL where no step is planned) */
+    uint32_t *n_free;     /* 1 */
+    int dev;              /* the device they are on */
+};
+
+/* What a step asks for, and what janas_attn_pages_plan answers. */
+struct janas_attn_plan {
+    const uint32_t *n_new; /* n_seqs: new tokens of each sequence, 0 allowed,
+                              or JANAS_ATTN_RELEASE */
+    uint32_t *len;         /* n_seqs: lengths after the step; may be the
+                              pool's own */
+    uint32_t *n_free;      /* 1: free pages after it; may be the pool's own */
+    uint32_t *granted;     /* n_seqs: n_new, or 0 where it was refused; may be
+                              n_new itself */
+    uint32_t *start;       /* n_seqs + 1: first packed row of each sequence's
+                              tokens (refused ones keep theirs), and their sum */
+    uint32_t *taken;       /* n_seqs + 1: pages taken before each sequence, and
+                              their sum */
+    uint32_t *slot;        /* max_tokens: page x (the pool's) page + row of each
+                              packed token; JANAS_ATTN_NONE for refused tokens
+                              and for rows behind the last token */
+    uint32_t *pos;         /* max_tokens: its position (0 where it has no slot) */
+    uint32_t *seq;         /* max_tokens: its sequence (0 behind the last) */
+    uint32_t max_tokens;   /* rows of the three; below 2^31 */
+};
+
+/*
+ * The step's pages and slots. Released pages (n_new JANAS_ATTN_RELEASE, the
+ * sequence's length becomes 0) go on top of the free ones, in the sequences'
+ * order; then each sequence takes ceil((len + n_new) / page) - ceil(len /
+ * page) pages from the top for its new blocks, written into its table row. A
+ * sequence is granted all of its tokens or none: none if they pass its table
+ * row (max_pages x page) or the packed rows (max_tokens), and, from the first
+ * one that finds too few free pages on, every sequence that needs one (those
+ * that need none go on). Of pages a table row names twice, or a table with
+ * entries outside the pool, nothing is checked here; no write leaves the
+ * arrays. n_free above n_pages counts as n_pages.
+ */
+int janas_attn_pages_plan(const struct janas_attn_pages *p,
+                          const struct janas_attn_plan *s, void *stream);
+
+/* The rows that a layer's q, k, v products leave of a step's tokens. */
+struct janas_attn_rows {
+    const float *k, *v;   /* n x n_kv x head_dim */
+    const float *q;       /* n x n_head x head_dim, or NULL: no queries */
+    float *q_out;         /* the prepared queries, packed; may be q itself
+                             where that is packed */
+    const float *k_norm, *q_norm; /* head_dim weights, or NULL: none */
+    const float *cs, *sn; /* n_tab x n_rot / 2: the rotation of each position */
+    const uint32_t *slot, *pos; /* n of each (janas_attn_pages_plan) */
+    float eps;
+    uint32_t n_rot, n_tab;
+    int v_norm;           /* values normalized without weights */
+    uint32_t n;           /* packed rows */
+    uint32_t n_head;      /* of q */
+    uint32_t k_stride, v_stride, q_stride; /* floats a token's row begins after
+                             the one before it; 0: packed */
+};
+
+/*
+ * The rows into their slots: keys normalized and turned, values optionally
+ * normalized, both written at the cache's type, and the queries normalized
+ * and turned into q_out - the arithmetic of janas_attn_cache_write and
+ * janas_attn_q_prep bit for bit, in one launch. A row whose slot is
+ * JANAS_ATTN_NONE or outside the pool, or whose position has no row of the
+ * table (n_rot above 0), is left out: nothing of it is written, its q_out
+ * row neither. Two rows with one slot are written in no order.
+ */
+int janas_attn_pages_write(const struct janas_attn_pages *p,
+                           const struct janas_attn_rows *r, void *stream);
+
+/*
+ * The key bounds of blocks. For each sequence the blocks that hold its last
+ * n_new[i] positions (a step's janas_attn_plan.granted; NULL: all its blocks)
+ * are computed anew from the cached keys up to its length, as half floats
+ * rounded outward and kept within +-65504 (NaN keys are passed over; a block
+ * of nothing else gets 65504, -65504). max_new: the largest n_new, for the
+ * launch's size only (0: not known).
+ */
+int janas_attn_pages_bounds(const struct janas_attn_pages *p,
+                            const uint32_t *n_new, uint32_t max_new,
+                            void *stream);
+
+/* A step's single tokens over the pool: the query of sequence i is row i of q
+   and its output row i of out - or, with row and granted, row row[i], and
+   sequences whose granted[i] is not 1 take no part (nothing of theirs is read
+   or written): janas_attn_plan's start and granted. row[i] at or past n_rows
+   takes no part either. */
+struct janas_attn_pages_call {
+    const float *q;          /* rows of n_head x head_dim */
+    float *out;              /* the same, packed */
+    const float *gate;       /* per the gate mode, packed, or NULL */
+    const uint32_t *row, *granted; /* n_seqs of each, or both NULL */
+    uint32_t n_rows;         /* rows of q, out and gate (with row) */
+    uint32_t q_stride;       /* floats a row of q begins after the one before
+                                it, a multiple of 4; 0: packed */
+    const uint32_t *sel;     /* n_seqs x n_kv x n_sel blocks, or NULL: all */
+    uint32_t n_sel;
+    void *work;              /* janas_attn_pages_work_bytes, 256-byte aligned;
+                                calls that may overlap need one each */
+    size_t work_bytes;
+    void *out_q8k;           /* or NULL: as janas_attn_seq's */
+};
+
+/* Device bytes that a janas_attn_pages_run or _select over p needs as work;
+   0 where the call would be refused. */
+size_t janas_attn_pages_work_bytes(const struct janas_attn *a,
+                                   const struct janas_attn_pages *p);
+
+/*
+ * Attention of one token of each sequence over its pages: the newest one, at
+ * position len - 1, sees positions max(0, len - window) .. len - 1, or those
+ * of them in its KV head's selected blocks: of the first min(n_sel, blocks of
+ * the sequence) entries, those below its block count (a block named twice
+ * counts twice). A row that sees nothing is 0. The instance gives heads, scale
+ * and window; its scores are FLOAT's whatever its way, float-accurate over
+ * every cache type: within 1e-5 of softmax-normalized outputs. A page outside
+ * the pool, or a length past the table row, makes the row NaN; nothing outside
+ * the arrays is read. How a sequence's positions are split depends on all
+ * the lengths of the call, so a row's last bits may differ from one batch to
+ * another (the same call gives the same bits). JANAS_ATTN_ENOTSUP: a ring, head
+ * sizes that janas_attn_run_dev_split refuses (f32 caches: above 256).
+ */
+int janas_attn_pages_run(struct janas_attn *a, const struct janas_attn_pages *p,
+                         int gate_mode, const struct janas_attn_pages_call *c,
+                         void *stream);
+
+/*
+ * The blocks each KV head's queries select, c->n_sel of them, into sel
+ * (n_seqs x n_kv x n_sel; c->sel is not read): of the blocks in sight, the first `first` and the last `last` ones, and of the
+ * others those with the largest scores, ascending, then JANAS_ATTN_NONE
+ * where there are fewer. A block's score is the largest that any of the group's
+ * queries could give a key inside the block's bounds: max over the heads of
+ * sum_d q_d x (q_d > 0 ? largest_d : smallest_d) (negated queries under a
+ * negative scale), summed in double and rounded to float; of equal scores the
+ * lower block. Needs bounds, first + last <= n_sel, max_pages up to 2^20; c's
+ * out, gate and out_q8k are not read. Rows of sequences that take no part stay
+ * as they are.
+ */
+int janas_attn_pages_select(struct janas_attn *a,
+                            const struct janas_attn_pages *p,
+                            const struct janas_attn_pages_call *c,
+                            uint32_t first, uint32_t last, uint32_t *sel,
+                            void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,7 @@
 
 #include "../../include/janas_attn.h"
 #include "attn_kernels.h"
+#include "attn_pages.h"
 
 using namespace janas;
 
@@ -1798,6 +1799,16 @@ extern "C" int janas_attn_run_dev_kernels(struct janas_attn *a, int kv_type,
     return note(a, run_split(a, kv_type, gate_mode, seqs, n_seqs,
                              stream ? (hipStream_t)stream : a->stream, kernels));
 }
+
+/* ===== what Part 4 uses of an instance (attn_pages_api.cpp) =========== */
+
+janas::PagesGeom janas::pages_geom(const janas_attn *a)
+{
+    return PagesGeom{a->n_head, a->n_kv, a->group, a->hd,   a->window,
+                     a->cus,    a->scale, a->ring, a->dev};
+}
+
+int janas::pages_note(janas_attn *a, int rc) { return note(a, rc); }
 
 extern "C" const char *janas_attn_strerror(int err)
 {

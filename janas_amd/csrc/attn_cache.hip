@@ -35,6 +35,7 @@
 #include <hip/hip_runtime.h>
 
 #include "attn_kernels.h"
+#include "attn_pages.h"
 #include "attn_q8k.h"
 
 namespace janas {
@@ -590,6 +591,148 @@ __global__ __launch_bounds__(256) void refresh_kernel(const RefreshArgs A)
     A.dst[t][((size_t)h * A.cap + row) * w + e] = A.src[t][i];
 }
 
+/* ---- a paged cache's rows ------------------------------------------------- */
+
+/* The place of token j in a pool: its slot and its row of the rotation's table;
+   false where it is left out */
+__device__ __forceinline__ bool page_row(const PagesRowArgs &A, uint32_t j, uint32_t &slot,
+                                         uint32_t &turn)
+{
+    slot = A.slot[j];
+    turn = A.n_rot ? A.pos[j] : 0;
+    return slot < A.n_slots && (A.n_rot == 0 || turn < A.n_tab);
+}
+
+/* cache row of KV head h in a slot: page, head, row of the page */
+__device__ __forceinline__ size_t page_at(const PagesRowArgs &A, uint32_t slot, uint32_t h)
+{
+    const size_t head = (size_t)(slot >> A.page_log) * A.n_kv + h;
+    return (head << A.page_log) + (slot & ((1u << A.page_log) - 1));
+}
+
+/*
+ * rows16_kernel's rows into slots: of each token n_kv key and value rows, then
+ * n_head query rows, 16 lanes a row. The slot and the position are read with
+ * the row's numbers; only the rotation's table waits for the position.
+ */
+template <int NB, int KV>
+__global__ __launch_bounds__(256) void pages_rows16_kernel(const PagesRowArgs A)
+{
+    __shared__ __attribute__((aligned(16))) float sR[kRowsWg][64 * NB];
+    const uint32_t c = threadIdx.x % kRowLanes, w = threadIdx.x / kRowLanes;
+    const uint64_t id = (uint64_t)blockIdx.x * kRowsWg + w;
+    const uint32_t heads = A.n_kv + A.n_head;
+    if (id >= (uint64_t)A.n * heads)
+        return;
+    const uint32_t j = (uint32_t)(id / heads), r = (uint32_t)(id % heads);
+    const uint32_t hd = A.hd, half = A.n_rot / 2;
+    const bool query = r >= A.n_kv;
+    const float *const src = query ? A.q + (size_t)j * A.q_stride + (size_t)(r - A.n_kv) * hd
+                                   : A.k + (size_t)j * A.k_stride + (size_t)r * hd;
+    const float *const vsrc = A.v + (size_t)j * A.v_stride + (size_t)r * hd;
+    const float *const norm = query ? A.q_norm : A.k_norm;
+    f4 k[NB], v[NB], nw[NB], cs[NB], sn[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const uint32_t col = 64 * b + 4 * c;
+        k[b] = v[b] = nw[b] = f4{0, 0, 0, 0};
+        if (col >= hd)
+            continue;
+        k[b] = *(const f4 *)(src + col);
+        if (!query)
+            v[b] = *(const f4 *)(vsrc + col);
+        if (norm)
+            nw[b] = *(const f4 *)(norm + col);
+    }
+    uint32_t slot, turn;
+    if (!page_row(A, j, slot, turn))
+        return;
+    load_table<NB>(A.cs + (size_t)turn * half, c, half, cs);
+    load_table<NB>(A.sn + (size_t)turn * half, c, half, sn);
+    if (norm) {
+        const float s = inv_rms16<NB>(k, hd, A.eps, A.inv_hd);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                k[b][e] = k[b][e] * s * nw[b][e];
+    }
+    rotate16<NB, false>(k, sR[w], c, hd, half, cs, sn);
+    if (query) {
+        float *const dst = A.q_out + ((size_t)j * A.n_head + (r - A.n_kv)) * hd;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+            if (64 * b + 4 * c < hd)
+                *(f4 *)(dst + 64 * b + 4 * c) = k[b];
+        return;
+    }
+    if (A.v_norm) {
+        const float s = inv_rms16<NB>(v, hd, A.eps, A.inv_hd);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[b][e] = v[b][e] * s;
+    }
+    const size_t at = page_at(A, slot, r);
+    constexpr size_t eb = KV == kI8 ? 1 : KV == kF32 ? 4 : 2;
+    put_row16<NB, KV>(k, c, hd, (char *)A.kc + at * hd * eb, A.kz + at);
+    put_row16<NB, KV>(v, c, hd, (char *)A.vc + at * hd * eb, A.vz + at);
+}
+
+/* The same for rows that are not whole aligned words: a wave a row */
+__global__ __launch_bounds__(64 * kRowWaves) void pages_rows_kernel(const PagesRowArgs A)
+{
+    __shared__ float sK[kRowWaves][kMaxHd], sV[kRowWaves][kMaxHd];
+    __shared__ float sS[kRowWaves];
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const uint64_t id = (uint64_t)blockIdx.x * kRowWaves + w;
+    const uint32_t heads = A.n_kv + A.n_head;
+    if (id >= (uint64_t)A.n * heads)
+        return;
+    const uint32_t j = (uint32_t)(id / heads), r = (uint32_t)(id % heads);
+    const uint32_t hd = A.hd, half = A.n_rot / 2;
+    uint32_t slot, turn;
+    if (!page_row(A, j, slot, turn))
+        return;
+    const bool query = r >= A.n_kv;
+    const float *const src = query ? A.q + (size_t)j * A.q_stride + (size_t)(r - A.n_kv) * hd
+                                   : A.k + (size_t)j * A.k_stride + (size_t)r * hd;
+    const float *const norm = query ? A.q_norm : A.k_norm;
+    float *kr = sK[w], *vr = sV[w];
+    for (uint32_t i = lane; i < hd; i += 64) {
+        kr[i] = src[i];
+        if (!query)
+            vr[i] = A.v[(size_t)j * A.v_stride + (size_t)r * hd + i];
+    }
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    if (norm) {
+        const float s = inv_rms(kr, hd, A.eps, lane, &sS[w]);
+        for (uint32_t i = lane; i < hd; i += 64)
+            kr[i] = kr[i] * s * norm[i];
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    rotate(kr, A.n_rot, A.cs + (size_t)turn * half, A.sn + (size_t)turn * half, lane, false);
+    if (query) {
+        for (uint32_t i = lane; i < hd; i += 64)
+            A.q_out[((size_t)j * A.n_head + (r - A.n_kv)) * hd + i] = kr[i];
+        return;
+    }
+    if (A.v_norm) {
+        const float s = inv_rms(vr, hd, A.eps, lane, &sS[w]);
+        for (uint32_t i = lane; i < hd; i += 64)
+            vr[i] = vr[i] * s;
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+    const size_t at = page_at(A, slot, r);
+    const size_t eb = A.kv == kI8 ? 1 : A.kv == kF32 ? 4 : 2;
+    quantize_row(kr, hd, A.kv, (char *)A.kc + at * hd * eb, A.kz ? A.kz + at : nullptr, lane);
+    quantize_row(vr, hd, A.kv, (char *)A.vc + at * hd * eb, A.vz ? A.vz + at : nullptr, lane);
+}
+
 }  // namespace
 
 hipError_t launch_refresh(const RefreshArgs &a, hipStream_t s)
@@ -652,6 +795,48 @@ hipError_t launch_rows(const RowArgs &a, hipStream_t s)
         return hipErrorInvalidValue;
     }
     hipLaunchKernelGGL(rows_kernel, dim3((rows + kRowWaves - 1) / kRowWaves),
+                       dim3(64 * kRowWaves), 0, s, a);
+    return hipGetLastError();
+}
+
+template <int KV> static void pages_rows16(const PagesRowArgs &a, dim3 grid, hipStream_t s)
+{
+    if (a.hd <= 64)
+        hipLaunchKernelGGL((pages_rows16_kernel<1, KV>), grid, dim3(256), 0, s, a);
+    else if (a.hd <= 128)
+        hipLaunchKernelGGL((pages_rows16_kernel<2, KV>), grid, dim3(256), 0, s, a);
+    else if (a.hd <= 256)
+        hipLaunchKernelGGL((pages_rows16_kernel<4, KV>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((pages_rows16_kernel<8, KV>), grid, dim3(256), 0, s, a);
+}
+
+hipError_t launch_pages_rows(const PagesRowArgs &a, hipStream_t s)
+{
+    const uint64_t rows = (uint64_t)a.n * (a.n_kv + a.n_head);
+    const size_t word = 4 * elem_size(a.kv);
+    if (a.hd % 4 == 0 && a.n_rot % 8 == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 &&
+        a.q_stride % 4 == 0 && aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.q, 16) &&
+        aligned(a.q_out, 16) && aligned(a.k_norm, 16) && aligned(a.q_norm, 16) &&
+        aligned(a.cs, 16) && aligned(a.sn, 16) && aligned(a.kc, word) && aligned(a.vc, word)) {
+        const dim3 grid((uint32_t)((rows + kRowsWg - 1) / kRowsWg));
+        switch (a.kv) {
+        case kI8:
+            pages_rows16<kI8>(a, grid, s);
+            break;
+        case kI16:
+            pages_rows16<kI16>(a, grid, s);
+            break;
+        case kF16:
+            pages_rows16<kF16>(a, grid, s);
+            break;
+        case kF32:
+            pages_rows16<kF32>(a, grid, s);
+            break;
+        }
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(pages_rows_kernel, dim3((uint32_t)((rows + kRowWaves - 1) / kRowWaves)),
                        dim3(64 * kRowWaves), 0, s, a);
     return hipGetLastError();
 }

@@ -1,0 +1,276 @@
+/*
+ * attn_pages_plan.hip - a serving step's pages and slots from the sequences'
+ * lengths, on the device: which free page each new block gets, and where each
+ * packed token's row goes.
+ *
+ * Two sums over the sequences decide everything: the tokens before a sequence
+ * (its first packed row) and the pages asked for before it (where in the stack
+ * of free pages its own begin). One workgroup takes them, 1024 sequences at a
+ * time, and for a small step (a decode's) writes tables and slots too: one
+ * launch. A large step's tokens and pages go to a second kernel, a thread each,
+ * which finds a token's sequence in the first rows by halving.
+ *
+ * Bound by its launches: a step of 48 sequences moves 2 KB.
+ */
+#include <stdint.h>
+
+#include <hip/hip_runtime.h>
+
+#include "attn_pages.h"
+
+namespace janas {
+namespace {
+
+constexpr uint32_t kPlanThreads = 1024;
+constexpr uint32_t kPlanWaves = kPlanThreads / 64;
+
+/* the sum of x over the threads before this one; total: over all */
+__device__ uint64_t scan_group(uint64_t x, uint64_t *lds, uint64_t &total)
+{
+    const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint64_t s = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t y = __shfl_up((unsigned long long)s, o, 64);
+        s += lane >= (uint32_t)o ? y : 0;
+    }
+    if (lane == 63)
+        lds[w] = s;
+    __syncthreads();
+    uint64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kPlanWaves; i++) {
+        const uint64_t y = lds[i];
+        before += i < w ? y : 0;
+        total += y;
+    }
+    __syncthreads();
+    return before + s - x;
+}
+
+__device__ __forceinline__ uint64_t blocks_of(uint64_t positions, uint32_t page_log)
+{
+    return (positions + (1u << page_log) - 1) >> page_log;
+}
+
+/* the page that is k-th from the top of a stack of `top` (0: outside it, never
+   read: a stack's count is checked against what is taken) */
+__device__ __forceinline__ uint32_t stack_page(const PlanArgs &A, uint64_t top, uint64_t k)
+{
+    return k < top ? A.free_pages[top - 1 - k] : 0;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs A)
+{
+    __shared__ uint64_t sScan[kPlanWaves];
+    __shared__ uint32_t sOld[kPlanThreads], sNew[kPlanThreads], sNeed[kPlanThreads];
+    __shared__ uint32_t sTok[kPlanThreads];
+    __shared__ uint64_t sTake[kPlanThreads];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint64_t room = (uint64_t)A.max_pages << A.page_log;
+    uint64_t top = *A.n_free;
+    top = top < A.n_pages ? top : A.n_pages;
+    /* every thread has the count before one of them may change it */
+    __syncthreads();
+
+    /* ---- released pages onto the stack, sequence after sequence ---- */
+    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += kPlanThreads) {
+        const uint32_t i = i0 + tid;
+        const bool gone = i < A.n_seqs && A.n_new[i] == kRelease;
+        if (!__syncthreads_or(gone))
+            continue;
+        uint64_t gave = 0, all;
+        if (gone) {
+            gave = blocks_of(A.len[i], A.page_log);
+            gave = gave < A.max_pages ? gave : A.max_pages;
+        }
+        const uint64_t at = top + scan_group(gave, sScan, all);
+        sNeed[tid] = (uint32_t)gave;
+        sTake[tid] = at;
+        __syncthreads();
+        for (uint32_t k = w; k < kPlanThreads && i0 + k < A.n_seqs; k += kPlanWaves) {
+            const uint32_t n = sNeed[k];
+            const uint32_t *const row = A.table + (size_t)(i0 + k) * A.max_pages;
+            for (uint32_t b = lane; b < n; b += 64)
+                if (sTake[k] + b < A.n_pages)
+                    A.free_pages[sTake[k] + b] = row[b];
+        }
+        top += all;
+        top = top < A.n_pages ? top : A.n_pages;
+        __syncthreads();
+    }
+    /* what was pushed is read below, by other threads */
+    __threadfence_block();
+    __syncthreads();
+
+    /* ---- tokens and pages ---- */
+    uint64_t tok = 0, asked = 0, took = 0;
+    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += kPlanThreads) {
+        const uint32_t i = i0 + tid;
+        uint64_t old = 0, add = 0, all_tok, all_need;
+        if (i < A.n_seqs) {
+            old = A.len[i];
+            add = A.n_new[i];
+            if (add == kRelease)
+                old = add = 0;
+        }
+        const uint64_t first = tok + scan_group(add, sScan, all_tok);
+        const bool fits = old + add <= room && first + add <= A.max_tokens;
+        const uint64_t have = blocks_of(old, A.page_log);
+        const uint64_t need = fits ? blocks_of(old + add, A.page_log) - have : 0;
+        const uint64_t before = asked + scan_group(need, sScan, all_need);
+        const bool ok = fits && (need == 0 || before + need <= top);
+        /* the pages taken up to here: once a sequence found too few, none */
+        uint64_t take = before;
+        uint64_t all_take = all_need;
+        if (asked + all_need > top) {
+            take = took + scan_group(ok ? need : 0, sScan, all_take);
+        }
+        if (i < A.n_seqs) {
+            A.start[i] = first < 0xFFFFFFFFu ? (uint32_t)first : 0xFFFFFFFFu;
+            A.taken[i] = (uint32_t)take;
+            A.granted[i] = ok ? (uint32_t)add : 0;
+            A.len_out[i] = (uint32_t)(old + (ok ? add : 0));
+        }
+        if (A.whole) {
+            const bool mine = i < A.n_seqs;
+            sOld[tid] = (uint32_t)old;
+            sNeed[tid] = ok ? (uint32_t)need : 0;
+            sTake[tid] = take;
+            sTok[tid] = first < A.max_tokens ? (uint32_t)first : A.max_tokens;
+            sNew[tid] = mine ? (add < A.max_tokens ? (uint32_t)add : A.max_tokens) : 0;
+            const bool many = mine && (add > 1 || need > 1);
+            if (mine && !many) {
+                /* a token or none, a page or none */
+                uint32_t *const row = A.table + (size_t)i * A.max_pages;
+                if (ok && need)
+                    row[have] = stack_page(A, top, take);
+                if (add && first < A.max_tokens) {
+                    uint32_t s = kNone;
+                    if (ok) {
+                        const uint32_t b = (uint32_t)old >> A.page_log;
+                        const uint32_t p = need ? stack_page(A, top, take) : row[b];
+                        s = (p << A.page_log) + ((uint32_t)old & ((1u << A.page_log) - 1));
+                    }
+                    A.slot[first] = s;
+                    A.pos[first] = ok ? (uint32_t)old : 0;
+                    A.seq[first] = i;
+                }
+            }
+            if (__syncthreads_or(many)) {
+                /* the others, a wave a sequence */
+                for (uint32_t k = w; k < kPlanThreads && i0 + k < A.n_seqs; k += kPlanWaves) {
+                    const uint32_t n = sNew[k], q = sNeed[k];
+                    if (n <= 1 && q <= 1)
+                        continue;
+                    const uint32_t at = sTok[k], o = sOld[k];
+                    const uint32_t h = (uint32_t)blocks_of(o, A.page_log);
+                    const bool given = (uint64_t)o + n <= room && A.granted[i0 + k] != 0;
+                    uint32_t *const row = A.table + (size_t)(i0 + k) * A.max_pages;
+                    for (uint32_t b = lane; b < q; b += 64)
+                        row[h + b] = stack_page(A, top, sTake[k] + b);
+                    for (uint32_t t = lane; t < n && at + t < A.max_tokens; t += 64) {
+                        uint32_t s = kNone, p = 0;
+                        if (given) {
+                            p = o + t;
+                            const uint32_t b = p >> A.page_log;
+                            s = b < h ? row[b] : stack_page(A, top, sTake[k] + b - h);
+                            s = (s << A.page_log) + (p & ((1u << A.page_log) - 1));
+                        }
+                        A.slot[at + t] = s;
+                        A.pos[at + t] = p;
+                        A.seq[at + t] = i0 + k;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        tok += all_tok;
+        asked += all_need;
+        took += all_take;
+    }
+    if (tid == 0) {
+        A.start[A.n_seqs] = tok < 0xFFFFFFFFu ? (uint32_t)tok : 0xFFFFFFFFu;
+        A.taken[A.n_seqs] = (uint32_t)took;
+        *A.n_free_out = (uint32_t)(top - took);
+    }
+    if (A.whole)
+        for (uint64_t t = tok + tid; t < A.max_tokens; t += kPlanThreads) {
+            A.slot[t] = kNone;
+            A.pos[t] = A.seq[t] = 0;
+        }
+}
+
+/* the last i of n with at[i] <= x (at[0] = 0) */
+__device__ __forceinline__ uint32_t last_at(const uint32_t *at, uint32_t n, uint32_t x)
+{
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (at[mid] <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+/* The tables' and the tokens' part of a large step: workgroups of 256 threads,
+   the first n_tok of them over tokens, the rest over taken pages. It reads
+   what plan_kernel left; a new block's page comes from the stack, not from the
+   table, which other workgroups write. */
+__global__ __launch_bounds__(256) void plan_fill_kernel(const PlanArgs A, uint32_t n_tok)
+{
+    const uint32_t took = A.taken[A.n_seqs];
+    const uint64_t top = (uint64_t)*A.n_free_out + took;
+    if (blockIdx.x >= n_tok) {
+        const uint32_t k = (blockIdx.x - n_tok) * 256 + threadIdx.x;
+        if (k >= took)
+            return;
+        const uint32_t i = last_at(A.taken, A.n_seqs, k);
+        const uint32_t h = (uint32_t)blocks_of(A.len_out[i] - A.granted[i], A.page_log);
+        A.table[(size_t)i * A.max_pages + h + (k - A.taken[i])] = stack_page(A, top, k);
+        return;
+    }
+    const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= A.max_tokens)
+        return;
+    uint32_t s = kNone, p = 0, i = 0;
+    if (t < A.start[A.n_seqs]) {
+        i = last_at(A.start, A.n_seqs, t);
+        const uint32_t n = A.granted[i];
+        if (n) {
+            const uint32_t old = A.len_out[i] - n;
+            const uint32_t h = (uint32_t)blocks_of(old, A.page_log);
+            p = old + (t - A.start[i]);
+            const uint32_t b = p >> A.page_log;
+            s = b < h ? A.table[(size_t)i * A.max_pages + b]
+                      : stack_page(A, top, (uint64_t)A.taken[i] + b - h);
+            s = (s << A.page_log) + (p & ((1u << A.page_log) - 1));
+        }
+    }
+    A.slot[t] = s;
+    A.pos[t] = p;
+    A.seq[t] = i;
+}
+
+}  // namespace
+
+hipError_t launch_plan(PlanArgs a, hipStream_t s)
+{
+    a.whole = a.max_tokens <= 4096;
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.whole)
+        return e;
+    const uint32_t n_tok = (a.max_tokens + 255) / 256;
+    /* a sequence's tokens take at most a page each, and one more a sequence */
+    uint64_t pages = ((uint64_t)a.max_tokens >> a.page_log) + a.n_seqs;
+    pages = pages < a.n_pages ? pages : a.n_pages;
+    const uint32_t n_page = (uint32_t)((pages + 255) / 256);
+    hipLaunchKernelGGL(plan_fill_kernel, dim3(n_tok + n_page), dim3(256), 0, s, a, n_tok);
+    return hipGetLastError();
+}
+
+}  // namespace janas
