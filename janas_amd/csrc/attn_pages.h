@@ -66,21 +66,27 @@ struct PagesArgs {
     const uint32_t *table, *len, *row, *granted, *sel;
     const float *q, *gate;
     float *out;
-    float *part_ml;        /* [n_wg][rows a workgroup][2] */
-    float *part_acc;       /* [n_wg][rows a workgroup][hd] */
+    float *part_ml;        /* [runs + n_seqs][tiles][rows a workgroup][2] */
+    float *part_acc;       /* the same of [hd]; tiles = n_kv x rtiles */
+    uint2 *plan;           /* [n_seqs]: a sequence's first partial and their
+                              count (kNone: it takes no part) */
     uint32_t n_seqs, n_rows, max_pages, n_pages, page_log, n_sel;
     uint32_t n_head, n_kv, group, hd, window, q_stride;
     uint32_t rtiles;       /* workgroups along a KV head's query rows */
-    uint32_t share;        /* splits a KV head's row tile aims at */
-    uint32_t n_wg;         /* (share + n_seqs) x n_kv x rtiles */
+    uint32_t share;        /* runs of a tile that the device holds at once */
+    uint32_t n_wg;         /* pages_runs x tiles; one more writes the plan */
     float scale;
     int gate_mode;
 };
 /* query rows a workgroup takes */
 inline uint32_t pages_rows_wg(int kv) { return kv == kF32 ? 16 : 8; }
 int pages_supported(int kv, uint32_t hd);
-/* the splits a KV head's row tile aims at, of `tiles` = n_kv x rtiles */
-uint32_t pages_share(uint32_t cus, uint32_t tiles);
+/* the runs of one of `tiles` = n_kv x rtiles that the device holds at once, and
+   the most that a call makes of them (most_units: a table row's) */
+uint32_t pages_share(int kv, uint32_t hd, uint32_t cus, uint32_t tiles);
+uint64_t pages_runs(uint32_t share, uint32_t n_seqs, uint64_t most_units);
+/* columns a merge workgroup takes */
+uint32_t pages_merge_cols(uint32_t n_seqs, uint32_t n_head, uint32_t hd);
 hipError_t launch_pages(int kv, const PagesArgs &a, hipStream_t s);
 hipError_t launch_pages_merge(int kv, const PagesArgs &a, hipStream_t s);
 

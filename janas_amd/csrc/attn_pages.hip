@@ -7,14 +7,15 @@
  * over the positions in sight, or those of a KV head's selected blocks.
  *
  *   pages_kernel   one workgroup (4 waves) per (sequence, KV head, tile of
- *                  query rows, split of the positions). A wave walks its own
- *                  positions in units of 16 - a page holds whole units - with
- *                  one running softmax; nothing is shared until the four waves
- *                  are joined at the end.
- *   pages_merge_kernel  joins a row's splits, in order, and applies the gate.
+ *                  query rows, run of positions). A wave walks its own positions
+ *                  in units of 16 - a page holds whole units - with one running
+ *                  softmax; nothing is shared until the four waves are joined
+ *                  at the end.
+ *   pages_merge_kernel  joins the partials of a row that several workgroups
+ *                  took, in order, and applies the gate.
  *
- * Both find their work on the device from the sequences' lengths (plan_splits),
- * so a launch depends on none and can be captured.
+ * The work is dealt on the device from the sequences' lengths (Runs), so a
+ * launch depends on none and can be captured.
  *
  * Operands go from memory to registers in the shape the matrix cores take
  * them, without LDS. Scores, S^T = K Q^T, contract over the head dimension in
@@ -30,6 +31,8 @@
  */
 #include <math.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include <hip/hip_runtime.h>
 
@@ -65,77 +68,119 @@ __device__ __forceinline__ uint32_t seq_units(const PagesArgs &A, const SeqView 
     }
 }
 
+/* the sum over the lanes up to and with this one: row_shr 1, 2, 4, 8 inside
+   rows of 16, then row_bcast 15 and 31 across them */
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t shifted(uint32_t x)
+{
+    return __builtin_amdgcn_update_dpp(0u, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x)
+{
+    x += shifted<0x111, 0xf>(x);
+    x += shifted<0x112, 0xf>(x);
+    x += shifted<0x114, 0xf>(x);
+    x += shifted<0x118, 0xf>(x);
+    x += shifted<0x142, 0xa>(x);
+    x += shifted<0x143, 0xc>(x);
+    return x;
+}
+__device__ __forceinline__ uint64_t uniform(uint64_t x)
+{
+    return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
+           __builtin_amdgcn_readfirstlane((uint32_t)x);
+}
 __device__ __forceinline__ uint32_t sum_wave(uint32_t x)
 {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        x += __shfl_xor(x, o, 64);
-    return x;
-}
-/* sum over the lanes up to and with this one */
-__device__ __forceinline__ uint32_t scan_wave(uint32_t x, uint32_t lane)
-{
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(x, o, 64);
-        x += lane >= (uint32_t)o ? y : 0;
-    }
-    return x;
+    return __builtin_amdgcn_readlane(scan_wave(x), 63);
 }
 
-/* units a split takes at least: 4 a wave. Below that a wave's start (length,
-   table, query, first rows: a chain of reads) is most of its time. */
-constexpr uint32_t kLeastUnits = 4 * kPW;
+/* units a workgroup takes at least: one a wave */
+constexpr uint32_t kLeastUnits = kPW;
 
-/* The units a split aims at: all sequences' units over the splits that a KV
-   head's row tile has (A.share). Every wave finds it for itself, a lane a
-   sequence. */
-template <bool SEL>
-__device__ __forceinline__ uint32_t split_units(const PagesArgs &A, uint32_t lane)
-{
-    uint64_t total = 0;
-    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        /* below 2^27 a lane (2^31 positions): 64 of them need a bit more */
-        const uint32_t u = i < A.n_seqs ? seq_units<SEL>(A, seq_view(A, i)) : 0;
-        total += (uint64_t)sum_wave(u >> 16) * 65536 + sum_wave(u & 0xFFFF);
-    }
-    const uint64_t per = (total + A.share - 1) / A.share;
-    return per < kLeastUnits ? kLeastUnits : per < 0xFFFFFFFFu ? (uint32_t)per : 0xFFFFFFFFu;
-}
-
-struct Split {
-    uint32_t seq, index, count, units; /* split `index` of `count`, of units */
+/*
+ * The work of a launch: the units of all sequences, one sequence after another,
+ * cut into runs of `per` - one a workgroup (of each KV head's row tile), A.share
+ * of them at most, which is what the device holds at once. Every workgroup then
+ * has the same number of units, whatever the lengths are, and one that crosses
+ * from a sequence into the next does one after the other. Where there are runs
+ * enough for it, each sequence begins a run of its own instead (its units
+ * rounded up to whole runs), so that no workgroup has two.
+ *
+ * Every wave finds its part for itself, a lane a sequence, 64 at a time; what it
+ * will want of them stays in LDS.
+ */
+struct RunsLds {
+    uint32_t row[64], lo[64], end[64], units[64];
+    uint64_t from[64], to[64];   /* a sequence's units in the launch's */
 };
 
-/* split number `at` of the call (per KV head and row tile), or the splits
-   before sequence `want` (index) and its own (count) */
-template <bool SEL>
-__device__ __forceinline__ Split find_split(const PagesArgs &A, uint32_t lane, uint32_t at,
-                                            uint32_t want)
-{
-    Split f{kNone, 0, 0, 0};
-    const uint32_t per = split_units<SEL>(A, lane);
-    uint32_t before = 0;
-    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        const uint32_t u = i < A.n_seqs ? seq_units<SEL>(A, seq_view(A, i)) : 0;
-        const uint32_t n = u ? (u - 1) / per + 1 : 0;
-        const uint32_t end = scan_wave(n, lane) + before;
-        const uint64_t past = want == kNone ? __ballot(end > at) : __ballot(i == want);
-        if (past) {
-            const uint32_t l = (uint32_t)__builtin_ctzll(past);
-            f.seq = i0 + l;
-            f.count = __builtin_amdgcn_readlane(n, l);
-            f.units = __builtin_amdgcn_readlane(u, l);
-            const uint32_t first = __builtin_amdgcn_readlane(end, l) - f.count;
-            f.index = want == kNone ? at - first : first;
-            return f;
-        }
-        before = __builtin_amdgcn_readlane(end, 63);
+template <bool SEL> struct Runs {
+    uint32_t i0, per, whole;     /* units a run; each sequence in whole runs */
+
+    static __device__ __forceinline__ uint32_t units(const PagesArgs &A, uint32_t i, SeqView &s)
+    {
+        s = SeqView{};
+        if (i >= A.n_seqs)
+            return 0;
+        s = seq_view(A, i);
+        return seq_units<SEL>(A, s);
     }
-    return f;
-}
+    /* sequences i0 .. i0 + 63, which follow on `before` units, to LDS */
+    __device__ __forceinline__ void place(const SeqView &s, uint32_t u, uint64_t before,
+                                          uint32_t lane, uint32_t w, RunsLds &L) const
+    {
+        const uint64_t r = whole && u ? (uint64_t)((u - 1) / per + 1) * per : u;
+        /* (64 lanes of less than 2^32: in halves) */
+        const uint64_t to = before + (uint64_t)scan_wave((uint32_t)(r >> 16)) * 65536 +
+                            scan_wave((uint32_t)r & 0xFFFF);
+        if (w == 0) {
+            L.row[lane] = s.part ? s.row : kNone;
+            L.lo[lane] = s.lo;
+            L.end[lane] = s.end;
+            L.units[lane] = u;
+            L.from[lane] = to - r;
+            L.to[lane] = to;
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ void begin(const PagesArgs &A, uint32_t lane, uint32_t w, RunsLds &L)
+    {
+        SeqView s;
+        uint32_t u = 0;
+        uint64_t total = 0;
+        for (i0 = 0; i0 < A.n_seqs; i0 += 64) {
+            u = units(A, i0 + lane, s);
+            total += (uint64_t)sum_wave(u >> 16) * 65536 + sum_wave(u & 0xFFFF);
+        }
+        uint64_t p = (total + A.share - 1) / A.share;
+        p = p < kLeastUnits ? kLeastUnits : p;
+        per = p < 0x10000000u ? (uint32_t)p : 0x10000000u;
+        uint64_t runs = 0;
+        for (i0 = 0; i0 < A.n_seqs; i0 += 64) {
+            if (A.n_seqs > 64)
+                u = units(A, i0 + lane, s);
+            runs += sum_wave(u ? (u - 1) / per + 1 : 0);
+        }
+        whole = runs <= A.share;
+        i0 = 0;
+        if (A.n_seqs > 64)
+            u = units(A, lane, s);
+        place(s, u, 0, lane, w, L);
+    }
+    /* the next 64 sequences; false: there are none */
+    __device__ __forceinline__ bool next(const PagesArgs &A, uint32_t lane, uint32_t w, RunsLds &L)
+    {
+        if (i0 + 64 >= A.n_seqs)
+            return false;
+        const uint64_t before = L.to[63];
+        __syncthreads();
+        i0 += 64;
+        SeqView s;
+        const uint32_t u = units(A, i0 + lane, s);
+        place(s, u, before, lane, w, L);
+        return true;
+    }
+};
 
 /* ---- raw words of a row ------------------------------------------------------ */
 
@@ -151,6 +196,15 @@ template <int W> __device__ __forceinline__ uint32_t word(const typename Words<W
         return x[i];
 }
 
+/* waves a SIMD that an instance's registers leave room for, and with that the
+   workgroups a compute unit holds */
+constexpr int pages_waves(int kv, int d)
+{
+    if (kv == kF32)
+        return d <= 64 ? 4 : d <= 128 ? 2 : 1;
+    return d <= 64 ? 4 : d <= 128 ? (kv == kI16 ? 3 : 4) : d <= 256 ? (kv == kI8 ? 3 : 2) : 1;
+}
+
 template <int T, int D> struct PS {
     static constexpr int EB = Elem<T>::bytes;
     static constexpr bool F32 = T == kF32;
@@ -162,6 +216,12 @@ template <int T, int D> struct PS {
     static constexpr int VW = VN * EB / 4;           /* words of one */
     static constexpr int NT = D / 16;                /* column tiles */
     static constexpr int DP = Elem<T>::planes;
+    /* the query's operands from head size 256 on are read from LDS at each use:
+       in registers they would cost a wave a SIMD (256) or spill (512) */
+    static constexpr bool QLDS = D >= 256;
+    static constexpr int QROW = F32 ? D + 4 : D / 2 + 4; /* words of an LDS row */
+    static constexpr int QCOLS = 16;
+    static constexpr int WAVES = pages_waves(T, D);  /* a SIMD, by registers */
 };
 
 /* numbers e of four rows' V words as B operands, one a plane */
@@ -211,7 +271,8 @@ __device__ __forceinline__ uint32_t exponent(float x) { return (__float_as_uint(
 /* ---- the kernel ---------------------------------------------------------------- */
 
 template <int T, int D, bool SEL>
-__global__ __launch_bounds__(kPW * 64) void pages_kernel(const PagesArgs A)
+__global__ __launch_bounds__(kPW * 64)
+__attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const PagesArgs A)
 {
     using S = PS<T, D>;
     constexpr int EB = S::EB, KL = S::KL, VN = S::VN, VU = S::VU, VW = S::VW, NT = S::NT;
@@ -221,408 +282,516 @@ __global__ __launch_bounds__(kPW * 64) void pages_kernel(const PagesArgs A)
     __shared__ __attribute__((aligned(16))) float sO[kPW][ROWS][D];
     __shared__ float sM[kPW][ROWS], sL[kPW][ROWS];
     __shared__ float sE[kPW];
+    __shared__ __attribute__((aligned(16))) float sQ[S::QLDS ? S::QCOLS : 1][S::QLDS ? S::QROW : 4];
+    __shared__ float sQs[ROWS];
+    __shared__ RunsLds sR;
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63;
-    const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t g = lane >> 4, n = lane & 15;
-    const uint32_t tiles = A.n_kv * A.rtiles, tile = blockIdx.x % tiles;
-    const Split sp = find_split<SEL>(A, lane, blockIdx.x / tiles, kNone);
-    if (sp.seq == kNone)
+    const uint32_t thread = threadIdx.x, w = __builtin_amdgcn_readfirstlane(thread >> 6);
+    const uint32_t tiles = A.n_kv * A.rtiles, tile = blockIdx.x % tiles, run = blockIdx.x / tiles;
+    Runs<SEL> R;
+    R.begin(A, thread & 63, w, sR);
+    if (blockIdx.x == A.n_wg) {
+        /* one workgroup more: for the merge, each sequence's partials - the one
+           of run x and sequence i has number x + i */
+        const uint32_t lane = thread & 63;
+        do {
+            const uint32_t i = R.i0 + lane, u = sR.units[lane];
+            const uint64_t r0 = sR.from[lane] / R.per;
+            const uint64_t r1 = u ? (sR.from[lane] + u - 1) / R.per + 1 : r0;
+            if (w == 0 && i < A.n_seqs)
+                A.plan[i] = make_uint2((uint32_t)r0 + i,
+                                       sR.row[lane] == kNone ? kNone : (uint32_t)(r1 - r0));
+        } while (R.next(A, lane, w, sR));
         return;
-    const SeqView sv = seq_view(A, sp.seq);
-    const uint32_t hd = A.hd, G = A.group, rowb = hd * EB;
-    const uint32_t kvh = tile / A.rtiles, r0 = tile % A.rtiles * ROWS;
-    const uint32_t rows = G - r0 < ROWS ? G - r0 : ROWS;
-    const uint32_t page = 1u << A.page_log, upp = page / kUnit, upp_log = A.page_log - 4;
-
-    /* the split's units, and the wave's quarter of them */
-    const uint32_t ua = (uint32_t)((uint64_t)sp.units * sp.index / sp.count);
-    const uint32_t ub = (uint32_t)((uint64_t)sp.units * (sp.index + 1) / sp.count);
-    const uint32_t wa = ua + (ub - ua) * w / kPW, wb = ua + (ub - ua) * (w + 1) / kPW;
-    /* units counted from the first page of the list */
-    const uint32_t u0 = SEL ? 0 : sv.lo / kUnit;
-    const uint32_t first = wa + u0, last = wb + u0; /* [first, last) */
-
-    /* ---- pages: lane i holds entry e0 + i of the wave's list - the block's page
-       and its number ---- */
-    const uint32_t nb = (sv.end + page - 1) >> A.page_log;
-    const uint32_t *const trow = A.table + (size_t)sp.seq * A.max_pages;
-    const uint32_t *const srow = SEL ? A.sel + ((size_t)sp.seq * A.n_kv + kvh) * A.n_sel : nullptr;
-    uint32_t e0 = first >> upp_log, pid = 0, blk = 0;
-    bool bad = false;
-    auto fetch = [&](uint32_t from) {
-        const uint32_t e = from + lane;
-        const bool mine = e <= (last - 1) >> upp_log;
-        blk = mine ? e : kNone;
-        if constexpr (SEL) {
-            if (mine)
-                blk = srow[e];
-        }
-        pid = 0;
-        if (blk < nb) {
-            pid = trow[blk];
-            bad |= pid >= A.n_pages;
-            pid = pid < A.n_pages ? pid : 0;
-        } else {
-            blk = kNone;
-        }
-    };
-
-    /* a unit: its page and KV head's rows, its first row and position (past
-       the end: none of it is in sight) */
-    struct Unit {
-        size_t row;
-        uint32_t pos;
-    };
-    auto unit_of = [&](uint32_t u) {
-        const uint32_t e = u >> upp_log;
-        if (e - e0 >= 64) {
-            e0 = e;
-            fetch(e0);
-        }
-        const uint32_t p = __builtin_amdgcn_readlane(pid, e - e0);
-        const uint32_t b = __builtin_amdgcn_readlane(blk, e - e0);
-        const uint32_t in = (u & (upp - 1)) * kUnit;
-        Unit x;
-        x.row = (((size_t)p * A.n_kv + kvh) << A.page_log) + in;
-        x.pos = b == kNone ? kNone - kUnit : (b << A.page_log) + in;
-        return x;
-    };
-
-    u4 kr[KL];
-    VT vr[4][VU];
-    f4 ks{1, 1, 1, 1}, vs{1, 1, 1, 1};
-    /* the lane's bytes of a K row, and its columns of a V row */
-    uint32_t kat[KL], vat[VU];
-    bool kback[KL];
-#pragma unroll
-    for (int i = 0; i < KL; i++) {
-        const uint32_t cb = 64 * i + 16 * g;
-        kback[i] = false;
-        if constexpr (EB == 1)
-            kat[i] = unit_at(cb, rowb, kback[i]);
-        else
-            kat[i] = cb < rowb ? cb : 0;
-        kat[i] += n * rowb;
     }
-#pragma unroll
-    for (int u = 0; u < VU; u++) {
-        const uint32_t c = 16 * VN * u + VN * n;
-        vat[u] = (c < hd ? c : 0) * EB;
-    }
-    auto load_k = [&](const Unit &x) {
-        const char *const p = (const char *)A.k + x.row * rowb;
-#pragma unroll
-        for (int i = 0; i < KL; i++)
-            kr[i] = __builtin_nontemporal_load((const u4 *)(p + kat[i]));
-        if constexpr (SCALED)
-            ks = *(const f4 *)(A.ks + x.row + 4 * g);
-    };
-    /* value rows past the sequence's are read as its last one (they weigh 0,
-       but what is there may be no number) */
-    auto load_v = [&](const Unit &x) {
-        const uint32_t hi = x.pos < sv.end ? (sv.end - 1 - x.pos < 15 ? sv.end - 1 - x.pos : 15) : 0;
-        const uint32_t lo = x.pos < sv.lo ? (sv.lo - x.pos < 15 ? sv.lo - x.pos : 15) : 0;
-        const char *const p = (const char *)A.v + x.row * rowb;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            uint32_t r = 4 * g + j;
-            r = r > lo ? r : lo;
-            r = r < hi ? r : hi;
-#pragma unroll
-            for (int u = 0; u < VU; u++)
-                vr[j][u] = __builtin_nontemporal_load((const VT *)(p + r * rowb + vat[u]));
-        }
-        if constexpr (SCALED)
-            vs = *(const f4 *)(A.vs + x.row + 4 * g);
-    };
+    uint64_t x0 = (uint64_t)run * R.per;
+    const uint64_t x1 = x0 + R.per;
+    /* sequence after sequence of the run */
+    for (;;) {
+        /* (the thread's number unknown to the compiler: what follows from it is made
+           anew for each sequence, not kept in registers across them) */
+        uint32_t tid = thread;
+        asm volatile("" : "+v"(tid));
+        const uint32_t lane = tid & 63, g = lane >> 4, n = lane & 15;
+        uint64_t hit;
+        while ((hit = __ballot(sR.units[lane] && sR.to[lane] > x0)) == 0)
+            if (!R.next(A, lane, w, sR))
+                return;
+        const uint32_t hl = (uint32_t)__builtin_ctzll(hit);
+        const uint32_t si = R.i0 + hl;
+        const uint32_t su = __builtin_amdgcn_readfirstlane(sR.units[hl]);
+        const uint64_t s0 = uniform(sR.from[hl]), s1 = uniform(sR.to[hl]);
+        if (s0 >= x1)
+            return;
+        SeqView sv;
+        sv.row = __builtin_amdgcn_readfirstlane(sR.row[hl]);
+        sv.lo = __builtin_amdgcn_readfirstlane(sR.lo[hl]);
+        sv.end = __builtin_amdgcn_readfirstlane(sR.end[hl]);
+        /* its units [ua, ub) are this run's; `only`: all of them */
+        const uint32_t ua = x0 > s0 ? (uint32_t)(x0 - s0) : 0;
+        const uint32_t ub = x1 - s0 < su ? (uint32_t)(x1 - s0) : su;
+        const bool only = ua == 0 && ub == su;
+        const uint32_t hd = A.hd, G = A.group, rowb = hd * EB;
+        const uint32_t kvh = tile / A.rtiles, r0 = tile % A.rtiles * ROWS;
+        const uint32_t rows = G - r0 < ROWS ? G - r0 : ROWS;
+        const uint32_t page = 1u << A.page_log, upp = page / kUnit, upp_log = A.page_log - 4;
 
-    /* ---- the query: row n / 2 (f32: n) as the B operand of each K load ---- */
-    constexpr int QN = 16 / EB;      /* numbers of a K load: 16, 8 or 4 */
-    h8 qb[F32 ? 1 : KL][F32 ? 1 : QN / 8];
-    f4 qf[F32 ? KL : 1];
-    float qs2;
-    {
-        const uint32_t qr = F32 ? n : n >> 1;
-        const bool ok = qr < rows;
-        const float *const src =
-            A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0 + (ok ? qr : 0)) * hd;
-        f4 x[KL][QN / 4];
-        float mx = 0.0f;
-#pragma unroll
-        for (int i = 0; i < KL; i++)
-#pragma unroll
-            for (int j = 0; j < QN / 4; j++) {
-                const uint32_t c = QN * (4 * i + g) + 4 * j;
-                x[i][j] = *(const f4 *)(src + (c < hd ? c : 0));
-                if (!ok || c >= hd)
-                    x[i][j] = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    mx = fmaxf(mx, fabsf(x[i][j][e]));
+        /* the wave's quarter of them */
+        const uint32_t wa = ua + (ub - ua) * w / kPW, wb = ua + (ub - ua) * (w + 1) / kPW;
+        /* units counted from the first page of the list */
+        const uint32_t u0 = SEL ? 0 : sv.lo / kUnit;
+        const uint32_t first = wa + u0, last = wb + u0; /* [first, last) */
+
+        /* ---- pages: lane i holds entry e0 + i of the wave's list - the block's page
+           and its number ---- */
+        const uint32_t nb = (sv.end + page - 1) >> A.page_log;
+        const uint32_t *const trow = A.table + (size_t)si * A.max_pages;
+        const uint32_t *const srow = SEL ? A.sel + ((size_t)si * A.n_kv + kvh) * A.n_sel : nullptr;
+        uint32_t e0 = first >> upp_log, pid = 0, blk = 0;
+        bool bad = false;            /* a page outside the pool */
+        auto fetch = [&](uint32_t from) {
+            const uint32_t e = from + lane;
+            const bool mine = e <= (last - 1) >> upp_log;
+            blk = mine ? e : kNone;
+            if constexpr (SEL) {
+                if (mine)
+                    blk = srow[e];
             }
-        if constexpr (F32) {
+            pid = 0;
+            if (blk < nb) {
+                pid = trow[blk];
+                bad |= pid >= A.n_pages;
+                pid = pid < A.n_pages ? pid : 0;
+            } else {
+                blk = kNone;
+            }
+        };
+
+        /* a unit: its page and KV head's rows, its first row and position (past
+           the end: none of it is in sight) */
+        struct Unit {
+            size_t row;
+            uint32_t pos;
+        };
+        auto unit_of = [&](uint32_t u) {
+            const uint32_t e = u >> upp_log;
+            if (e - e0 >= 64) {
+                e0 = e;
+                fetch(e0);
+            }
+            const uint32_t p = __builtin_amdgcn_readlane(pid, e - e0);
+            const uint32_t b = __builtin_amdgcn_readlane(blk, e - e0);
+            const uint32_t in = (u & (upp - 1)) * kUnit;
+            Unit x;
+            x.row = (((size_t)p * A.n_kv + kvh) << A.page_log) + in;
+            x.pos = b == kNone ? kNone - kUnit : (b << A.page_log) + in;
+            return x;
+        };
+
+        u4 kr[KL];
+        VT vr[4][VU];
+        f4 ks{1, 1, 1, 1}, vs{1, 1, 1, 1};
+        /* the lane's bytes of a K row, and its columns of a V row */
+        uint32_t kat[KL], vat[VU];
+        bool kback[KL];
+#pragma unroll
+        for (int i = 0; i < KL; i++) {
+            const uint32_t cb = 64 * i + 16 * g;
+            kback[i] = false;
+            if constexpr (EB == 1)
+                kat[i] = unit_at(cb, rowb, kback[i]);
+            else
+                kat[i] = cb < rowb ? cb : 0;
+            kat[i] += n * rowb;
+        }
+#pragma unroll
+        for (int u = 0; u < VU; u++) {
+            const uint32_t c = 16 * VN * u + VN * n;
+            vat[u] = (c < hd ? c : 0) * EB;
+        }
+        auto load_k = [&](const Unit &x) {
+            const char *const p = (const char *)A.k + x.row * rowb;
 #pragma unroll
             for (int i = 0; i < KL; i++)
-                qf[i] = x[i][0];
-            qs2 = A.scale * kLog2e;
-        } else {
-            /* scaled by 2^ex so that the row's largest lies in [2^13, 2^14);
-               even columns take the high plane, odd ones what is left */
-            mx = max_x32(max_x16(mx));
-            int ex = 0;
+                kr[i] = __builtin_nontemporal_load((const u4 *)(p + kat[i]));
+            if constexpr (SCALED)
+                ks = *(const f4 *)(A.ks + x.row + 4 * g);
+        };
+        /* value rows past the sequence's are read as its last one (they weigh 0,
+           but what is there may be no number) */
+        auto load_v = [&](const Unit &x) {
+            const uint32_t hi = x.pos < sv.end ? (sv.end - 1 - x.pos < 15 ? sv.end - 1 - x.pos : 15) : 0;
+            const uint32_t lo = x.pos < sv.lo ? (sv.lo - x.pos < 15 ? sv.lo - x.pos : 15) : 0;
+            const char *const p = (const char *)A.v + x.row * rowb;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                uint32_t r = 4 * g + j;
+                r = r > lo ? r : lo;
+                r = r < hi ? r : hi;
+#pragma unroll
+                for (int u = 0; u < VU; u++)
+                    vr[j][u] = __builtin_nontemporal_load((const VT *)(p + r * rowb + vat[u]));
+            }
+            if constexpr (SCALED)
+                vs = *(const f4 *)(A.vs + x.row + 4 * g);
+        };
+
+        /* ---- the query: MFMA column n's (row n / 2, plane n & 1; f32: row n) as the
+           B operand of each K load, in registers or LDS. Planes: scaled by 2^ex so
+           that the row's largest lies in [2^13, 2^14) ---- */
+        constexpr int QN = 16 / EB;      /* numbers of a K load: 16, 8 or 4 */
+        constexpr bool QLDS = S::QLDS;
+        u4 qr[QLDS ? 1 : KL][QLDS ? 1 : EB == 1 ? 2 : 1];
+        float qs2;
+        auto plane_scale = [](float mx, int &ex) {
+            ex = 0;
             if (mx > 0.0f && mx < INFINITY) {
                 frexpf(mx, &ex);
                 ex = 14 - ex;
             }
-            const float up = ldexpf(1.0f, ex);
+            return ldexpf(1.0f, ex);
+        };
+        if constexpr (QLDS) {
+            /* the workgroup's rows once: 256 / ROWS lanes a row, words of four */
+            constexpr int TPR = kPW * 64 / ROWS, NQ = D / (4 * TPR);
+            const uint32_t r = tid / TPR, t = tid % TPR;
+            const bool ok = r < rows;
+            const float *const src =
+                A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0 + (ok ? r : 0)) * hd;
+            f4 x[NQ];
+            float mx = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NQ; j++) {
+                const uint32_t c = 4 * (t + TPR * j);
+                x[j] = *(const f4 *)(src + (c < hd ? c : 0));
+                if (!ok || c >= hd)
+                    x[j] = f4{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    mx = fmaxf(mx, fabsf(x[j][e]));
+            }
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < NQ; j++)
+                    *(f4 *)&sQ[r][4 * (t + TPR * j)] = x[j];
+            } else {
+                mx = max_x16(max_row16(mx));
+                int ex;
+                const float up = plane_scale(mx, ex);
+#pragma unroll
+                for (int j = 0; j < NQ; j++) {
+                    h4 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        _Float16 a, b;
+                        split_hl(x[j][e] * up, a, b);
+                        hi[e] = a;
+                        lo[e] = b;
+                    }
+                    *(h4 *)&sQ[2 * r][2 * (t + TPR * j)] = hi;
+                    *(h4 *)&sQ[2 * r + 1][2 * (t + TPR * j)] = lo;
+                }
+                if (t == 0)
+                    sQs[r] = ldexpf(1.0f, -ex);
+            }
+            __syncthreads();
+            qs2 = F32 ? 1.0f : sQs[n >> 1];
+        } else {
+            const uint32_t qrow = F32 ? n : n >> 1;
+            const bool ok = qrow < rows;
+            const float *const src =
+                A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0 + (ok ? qrow : 0)) * hd;
+            f4 x[KL][QN / 4];
+            float mx = 0.0f;
 #pragma unroll
             for (int i = 0; i < KL; i++)
 #pragma unroll
-                for (int j = 0; j < QN / 4; j++)
+                for (int j = 0; j < QN / 4; j++) {
+                    const uint32_t c = QN * (4 * i + g) + 4 * j;
+                    x[i][j] = *(const f4 *)(src + (c < hd ? c : 0));
+                    if (!ok || c >= hd)
+                        x[i][j] = f4{0, 0, 0, 0};
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        _Float16 hi, lo;
-                        split_hl(x[i][j][e] * up, hi, lo);
-                        qb[i][j / 2][4 * (j & 1) + e] = n & 1 ? lo : hi;
-                    }
-            qs2 = ldexpf(1.0f, -ex) * A.scale * kLog2e;
-        }
-    }
-
-    /* ---- the wave's positions ---- */
-    f4 o[NT];
-#pragma unroll
-    for (int t = 0; t < NT; t++)
-        o[t] = f4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;  /* of the lane's row; l its own positions' */
-    uint32_t ev = 64;               /* exponent field that the value scales stay
-                                       within */
-    float vup = 0.0f;               /* a weight's factor: 2^kUp over theirs */
-    const float keep = lane & 1 ? -1.0f : -0.0f;
-    if (first < last) {
-        fetch(e0);
-        Unit x = unit_of(first);
-        load_k(x);
-        load_v(x);
-        for (uint32_t u = first; u < last; u++) {
-            const Unit now = x;
-            const bool more = u + 1 < last;
-            if (more)
-                x = unit_of(u + 1);
-            /* scores: lane holds positions 4 g + j of MFMA column n */
-            f4 s{0, 0, 0, 0};
+                    for (int e = 0; e < 4; e++)
+                        mx = fmaxf(mx, fabsf(x[i][j][e]));
+                }
+            int ex = 0;
+            const float up = plane_scale(max_x32(max_x16(mx)), ex);
 #pragma unroll
             for (int i = 0; i < KL; i++) {
                 if constexpr (F32) {
-                    const f4 kf = __builtin_bit_cast(f4, kr[i]);
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[i][e], s, 0, 0, 0);
-                } else if constexpr (T == kI8) {
-                    const u4 y = unit_fix(kr[i], kback[i]);
-                    s = mfma(i8_widen8(y.x, y.y), qb[i][0], s);
-                    s = mfma(i8_widen8(y.z, y.w), qb[i][1], s);
-                } else if constexpr (T == kI16) {
-                    h8 hi, lo;
-                    i16_planes8(kr[i].x, kr[i].y, kr[i].z, kr[i].w, hi, lo);
-                    s = mfma(hi, qb[i][0], s);
-                    s = mfma(lo, qb[i][0], s);
+                    qr[i][0] = __builtin_bit_cast(u4, x[i][0]);
                 } else {
-                    s = mfma(__builtin_bit_cast(h8, kr[i]), qb[i][0], s);
+#pragma unroll
+                    for (int j = 0; j < QN / 8; j++) {
+                        h8 y;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            _Float16 hi, lo;
+                            split_hl(x[i][2 * j + e / 4][e & 3] * up, hi, lo);
+                            y[e] = n & 1 ? lo : hi;
+                        }
+                        qr[i][j] = __builtin_bit_cast(u4, y);
+                    }
                 }
             }
-            const f4 kz = ks;
-            if (more)
-                load_k(x);
-            if (now.pos < sv.end && now.pos + kUnit > sv.lo) {
-                f4 vz = vs;
+            qs2 = F32 ? 1.0f : ldexpf(1.0f, -ex);
+        }
+        qs2 = qs2 * A.scale * kLog2e;
+        /* operand j of K load i; `at`: the lane's place in LDS, unknown to the
+           compiler from unit to unit, so that the reads stay in the loop */
+        auto q_operand = [&](int i, int j, uint32_t place) {
+            if constexpr (QLDS)
+                return *(const u4 *)((const char *)&sQ[0][0] + place + 64 * (EB == 1 ? 2 : 1) * i +
+                                     16 * j);
+            else
+                return qr[i][j];
+        };
+
+        /* ---- the wave's positions ---- */
+        f4 o[NT];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if constexpr (!F32)
-                        s[j] += from_x1(s[j]);
-                    s[j] *= qs2;
-                    if constexpr (SCALED)
-                        s[j] *= kz[j];
+        for (int t = 0; t < NT; t++)
+            o[t] = f4{0, 0, 0, 0};
+        float m = -INFINITY, l = 0.0f;  /* of the lane's row; l its own positions' */
+        uint32_t ev = 64;               /* exponent field that the value scales stay
+                                           within */
+        float vup = 0.0f;               /* a weight's factor: 2^kUp over theirs */
+        const float keep = lane & 1 ? -1.0f : -0.0f;
+        if (first < last) {
+            fetch(e0);
+            Unit x = unit_of(first);
+            load_k(x);
+            load_v(x);
+            for (uint32_t u = first; u < last; u++) {
+                const Unit now = x;
+                const bool more = u + 1 < last;
+                if (more)
+                    x = unit_of(u + 1);
+                /* scores: lane holds positions 4 g + j of MFMA column n */
+                f4 s{0, 0, 0, 0};
+                uint32_t place = n * S::QROW * 4 + 16 * (EB == 1 ? 2 : 1) * g;
+                if constexpr (QLDS)
+                    asm volatile("" : "+v"(place));
+#pragma unroll
+                for (int i = 0; i < KL; i++) {
+                    const u4 q0 = q_operand(i, 0, place);
+                    if constexpr (F32) {
+                        const f4 kf = __builtin_bit_cast(f4, kr[i]), qf = __builtin_bit_cast(f4, q0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s, 0, 0, 0);
+                    } else if constexpr (T == kI8) {
+                        const u4 y = unit_fix(kr[i], kback[i]);
+                        s = mfma(i8_widen8(y.x, y.y), __builtin_bit_cast(h8, q0), s);
+                        s = mfma(i8_widen8(y.z, y.w), __builtin_bit_cast(h8, q_operand(i, 1, place)), s);
+                    } else if constexpr (T == kI16) {
+                        h8 hi, lo;
+                        i16_planes8(kr[i].x, kr[i].y, kr[i].z, kr[i].w, hi, lo);
+                        s = mfma(hi, __builtin_bit_cast(h8, q0), s);
+                        s = mfma(lo, __builtin_bit_cast(h8, q0), s);
+                    } else {
+                        s = mfma(__builtin_bit_cast(h8, kr[i]), __builtin_bit_cast(h8, q0), s);
+                    }
                 }
-                if (now.pos < sv.lo || now.pos + kUnit > sv.end) {
+                const f4 kz = ks;
+                if (more)
+                    load_k(x);
+                if (now.pos < sv.end && now.pos + kUnit > sv.lo) {
+                    f4 vz = vs;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const uint32_t p = now.pos + 4 * g + j;
-                        const bool in = p >= sv.lo && p < sv.end;
-                        s[j] = in ? s[j] : -INFINITY;
-                        vz[j] = in ? vz[j] : 0.0f;
-                    }
-                }
-                const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-                uint32_t ex = 0;
-                if constexpr (SCALED)
-                    ex = exponent(fmaxf(fmaxf(vz[0], vz[1]), fmaxf(vz[2], vz[3])));
-                if (__any(top > m + kLazy || ex > ev)) {
-                    /* new references; what is summed so far follows */
-                    const float mn = fmaxf(m, max_x32(max_x16(top)));
-                    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                    m = mn;
-                    l *= f;
-                    float fe = 1.0f;
-                    if constexpr (SCALED) {
-                        const uint32_t en = (uint32_t)fmaxf((float)ev, max_x32(max_x16((float)ex)));
-                        fe = ldexpf(1.0f, (int)ev - (int)en);
-                        ev = en;
-                    }
-                    vup = ldexpf(1.0f, kUp + (SCALED ? 126 - (int)ev : 0));
-                    float fr[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        fr[i] = __shfl(f, (int)(4 * g + (F32 ? i : i & 2)), 64) * fe;
-#pragma unroll
-                    for (int t = 0; t < NT; t++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            o[t][i] *= fr[i];
-                }
-                const float mm = m == -INFINITY ? 0.0f : m;
-                h4 pa;
-                f4 pf;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float p = __builtin_amdgcn_exp2f(s[j] - mm);
-                    l += p;
-                    pf[j] = p;
-                    if constexpr (!F32) {
-                        float pv = p * vup;
+                        if constexpr (!F32)
+                            s[j] += from_x1(s[j]);
+                        s[j] *= qs2;
                         if constexpr (SCALED)
-                            pv *= vz[j];
-                        asm volatile("" : "+v"(pv));
-                        const float hi = (float)(_Float16)pv;
-                        pa[j] = (_Float16)__builtin_fmaf(keep, hi, pv);
+                            s[j] *= kz[j];
                     }
-                }
-                /* values: product e of a unit of columns */
+                    if (now.pos < sv.lo || now.pos + kUnit > sv.end) {
 #pragma unroll
-                for (int c = 0; c < VU; c++)
-#pragma unroll
-                    for (int e = 0; e < VN; e++) {
-                        const int t = c * VN + e;
-                        if constexpr (F32) {
-#pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    pf[j], __uint_as_float(word<VW>(vr[j][c], e)), o[t], 0, 0, 0);
-                        } else {
-                            const VT v4[4] = {vr[0][c], vr[1][c], vr[2][c], vr[3][c]};
-                            h4 vb[DP];
-                            value_operand<T, VW>(v4, e, vb);
-#pragma unroll
-                            for (int d = 0; d < DP; d++)
-                                o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, vb[d], o[t], 0, 0, 0);
+                        for (int j = 0; j < 4; j++) {
+                            const uint32_t p = now.pos + 4 * g + j;
+                            const bool in = p >= sv.lo && p < sv.end;
+                            s[j] = in ? s[j] : -INFINITY;
+                            vz[j] = in ? vz[j] : 0.0f;
                         }
                     }
+                    const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+                    uint32_t ex = 0;
+                    if constexpr (SCALED)
+                        ex = exponent(fmaxf(fmaxf(vz[0], vz[1]), fmaxf(vz[2], vz[3])));
+                    if (__any(top > m + kLazy || ex > ev)) {
+                        /* new references; what is summed so far follows */
+                        const float mn = fmaxf(m, max_x32(max_x16(top)));
+                        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                        m = mn;
+                        l *= f;
+                        float fe = 1.0f;
+                        if constexpr (SCALED) {
+                            const uint32_t en = (uint32_t)fmaxf((float)ev, max_x32(max_x16((float)ex)));
+                            fe = ldexpf(1.0f, (int)ev - (int)en);
+                            ev = en;
+                        }
+                        vup = ldexpf(1.0f, kUp + (SCALED ? 126 - (int)ev : 0));
+                        float fr[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            fr[i] = __shfl(f, (int)(4 * g + (F32 ? i : i & 2)), 64) * fe;
+#pragma unroll
+                        for (int t = 0; t < NT; t++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++)
+                                o[t][i] *= fr[i];
+                    }
+                    const float mm = m == -INFINITY ? 0.0f : m;
+                    h4 pa;
+                    f4 pf;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float p = __builtin_amdgcn_exp2f(s[j] - mm);
+                        l += p;
+                        pf[j] = p;
+                        if constexpr (!F32) {
+                            float pv = p * vup;
+                            if constexpr (SCALED)
+                                pv *= vz[j];
+                            asm volatile("" : "+v"(pv));
+                            const float hi = (float)(_Float16)pv;
+                            pa[j] = (_Float16)__builtin_fmaf(keep, hi, pv);
+                        }
+                    }
+                    /* values: product e of a unit of columns */
+#pragma unroll
+                    for (int c = 0; c < VU; c++)
+#pragma unroll
+                        for (int e = 0; e < VN; e++) {
+                            const int t = c * VN + e;
+                            if constexpr (F32) {
+#pragma unroll
+                                for (int j = 0; j < 4; j++)
+                                    o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                        pf[j], __uint_as_float(word<VW>(vr[j][c], e)), o[t], 0, 0, 0);
+                            } else {
+                                const VT v4[4] = {vr[0][c], vr[1][c], vr[2][c], vr[3][c]};
+                                h4 vb[DP];
+                                value_operand<T, VW>(v4, e, vb);
+#pragma unroll
+                                for (int d = 0; d < DP; d++)
+                                    o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, vb[d], o[t], 0, 0, 0);
+                            }
+                        }
+                }
+                if (more)
+                    load_v(x);
             }
-            if (more)
-                load_v(x);
         }
-    }
 
-    /* ---- the waves joined ---- */
-    l = sum_x32(sum_x16(l));
-    if (__any(bad))
-        l = NAN;
-    if (F32 ? lane < 16 : lane < 16 && !(lane & 1)) {
-        const uint32_t r = F32 ? lane : lane >> 1;
-        /* a bad wave may have no score of its own */
-        sM[w][r] = l != l && m == -INFINITY ? 0.0f : m;
-        sL[w][r] = l;
-    }
-    if (lane == 0)
-        sE[w] = F32 ? 1.0f : ldexpf(1.0f, -kUp - (SCALED ? 126 - (int)ev : 0));
+        /* ---- the waves joined ---- */
+        l = sum_x32(sum_x16(l));
+        if (__any(bad))
+            l = NAN;
+        if (F32 ? lane < 16 : lane < 16 && !(lane & 1)) {
+            const uint32_t r = F32 ? lane : lane >> 1;
+            /* a bad wave may have no score of its own */
+            sM[w][r] = l != l && m == -INFINITY ? 0.0f : m;
+            sL[w][r] = l;
+        }
+        if (lane == 0)
+            sE[w] = F32 ? 1.0f : ldexpf(1.0f, -kUp - (SCALED ? 126 - (int)ev : 0));
 #pragma unroll
-    for (int c = 0; c < VU; c++)
+        for (int c = 0; c < VU; c++)
 #pragma unroll
-        for (int i = 0; i < (F32 ? 4 : 2); i++) {
-            const uint32_t r = F32 ? 4 * g + i : 2 * g + i;
-            if (r >= rows)
+            for (int i = 0; i < (F32 ? 4 : 2); i++) {
+                const uint32_t r = F32 ? 4 * g + i : 2 * g + i;
+                if (r >= rows)
+                    continue;
+                float y[VN];
+#pragma unroll
+                for (int e = 0; e < VN; e++)
+                    y[e] = F32 ? o[c * VN + e][i] : o[c * VN + e][2 * i] + o[c * VN + e][2 * i + 1];
+#pragma unroll
+                for (int e = 0; e < VN; e += 4)
+                    *(f4 *)&sO[w][r][16 * VN * c + VN * n + e] = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+            }
+        __syncthreads();
+        const uint32_t c4 = hd / 4;      /* (hd: a multiple of 8) */
+        for (uint32_t t = tid; t < rows * c4; t += kPW * 64) {
+            const uint32_t r = t / c4, c = 4 * (t % c4);
+            const float mx = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
+            f4 y{0, 0, 0, 0};
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kPW; i++) {
+                const float f = sM[i][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[i][r] - mx);
+                sum += f * sL[i][r];
+                const f4 x = *(const f4 *)&sO[i][r][c];
+                const float fo = f * sE[i];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    y[e] += fo * x[e];
+            }
+            if (!only) {
+                const size_t pr = ((size_t)(run + si) * tiles + tile) * ROWS + r;
+                *(f4 *)(A.part_acc + pr * hd + c) = y;
+                if (c == 0)
+                    *(float2 *)(A.part_ml + 2 * pr) = make_float2(mx, sum);
                 continue;
-            float y[VN];
+            }
+            const size_t hr = (size_t)sv.row * A.n_head + kvh * G + r0 + r;
+            /* (nothing in sight, in selected blocks: 0) */
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            f4 sg{1, 1, 1, 1};
+            if (A.gate_mode == kGateElem)
+                sg = *(const f4 *)(A.gate + hr * hd + c);
+            else if (A.gate_mode == kGateHead)
+                sg[0] = sg[1] = sg[2] = sg[3] = A.gate[hr];
 #pragma unroll
-            for (int e = 0; e < VN; e++)
-                y[e] = F32 ? o[c * VN + e][i] : o[c * VN + e][2 * i] + o[c * VN + e][2 * i + 1];
-#pragma unroll
-            for (int e = 0; e < VN; e += 4)
-                *(f4 *)&sO[w][r][16 * VN * c + VN * n + e] = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+            for (int e = 0; e < 4; e++) {
+                y[e] *= inv;
+                if (A.gate_mode != kGateNone)
+                    y[e] *= sigmoid(sg[e]);
+            }
+            *(f4 *)(A.out + hr * hd + c) = y;
         }
-    __syncthreads();
-    const uint32_t c4 = hd / 4;      /* (hd: a multiple of 8) */
-    for (uint32_t t = tid; t < rows * c4; t += kPW * 64) {
-        const uint32_t r = t / c4, c = 4 * (t % c4);
-        const float mx = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
-        f4 y{0, 0, 0, 0};
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kPW; i++) {
-            const float f = sM[i][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[i][r] - mx);
-            sum += f * sL[i][r];
-            const f4 x = *(const f4 *)&sO[i][r][c];
-            const float fo = f * sE[i];
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                y[e] += fo * x[e];
-        }
-        if (sp.count > 1) {
-            const size_t pr = (size_t)blockIdx.x * ROWS + r;
-            *(f4 *)(A.part_acc + pr * hd + c) = y;
-            if (c == 0)
-                *(float2 *)(A.part_ml + 2 * pr) = make_float2(mx, sum);
-            continue;
-        }
-        const size_t hr = (size_t)sv.row * A.n_head + kvh * G + r0 + r;
-        /* (nothing in sight, in selected blocks: 0) */
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-        f4 sg{1, 1, 1, 1};
-        if (A.gate_mode == kGateElem)
-            sg = *(const f4 *)(A.gate + hr * hd + c);
-        else if (A.gate_mode == kGateHead)
-            sg[0] = sg[1] = sg[2] = sg[3] = A.gate[hr];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            y[e] *= inv;
-            if (A.gate_mode != kGateNone)
-                y[e] *= sigmoid(sg[e]);
-        }
-        *(f4 *)(A.out + hr * hd + c) = y;
+        x0 = s1;
+        if (x0 >= x1)
+            return;
+        __syncthreads(); /* (the next sequence's rows take the same LDS) */
     }
 }
 
 /* ---- the merge --------------------------------------------------------------- */
 
-constexpr uint32_t kMCols = 32;              /* columns a workgroup */
-constexpr uint32_t kMLanes = kMCols / 4;     /* lanes of a split: a float4 each */
-constexpr uint32_t kMGroups = 256 / kMLanes; /* splits at once */
 constexpr int kMBatch = 4;
 
-/* A row's splits joined: group i of 32 takes splits i, i + 32, ... with a
-   running maximum, the groups of a wave and then the waves are joined in a
-   fixed tree. Rows of one split are written by pages_kernel, rows that see
-   nothing here: 0, or NaN where the length passes the table. */
-template <bool SEL, int ROWS> __global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
+/*
+ * A row's splits joined, COLS columns a workgroup: COLS / 4 lanes take a split
+ * (a float4 each), so 1024 / COLS splits go at once, group i taking splits i, i
+ * + groups, ... with a running maximum; the groups of a wave and then the waves
+ * are joined in a fixed tree. Rows of one split are pages_kernel's; rows that
+ * see nothing are written here: 0, or NaN where the length passes the table.
+ * 32 columns where there are few rows (many splits each, and the device to
+ * fill), 128 where there are many (pages_merge_cols).
+ */
+template <int ROWS, int COLS>
+__global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
 {
+    constexpr uint32_t LANES = COLS / 4, GROUPS = 256 / LANES;
     __shared__ float sM[4], sL[4];
-    __shared__ f4 sA[4][kMLanes];
+    __shared__ f4 sA[4][LANES];
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t hd = A.hd, nd = (hd + kMCols - 1) / kMCols;
+    const uint32_t hd = A.hd, nd = (hd + COLS - 1) / COLS;
     const uint32_t h = blockIdx.x / nd % A.n_head, si = blockIdx.x / nd / A.n_head;
-    const uint32_t col = blockIdx.x % nd * kMCols + 4 * (lane % kMLanes);
-    const SeqView sv = seq_view(A, si);
-    if (!sv.part)
+    const uint32_t col = blockIdx.x % nd * COLS + 4 * (lane % LANES);
+    const uint2 plan = A.plan[si];
+    const uint32_t first = plan.x, count = plan.y;
+    if (count == kNone || count == 1)
         return;
-    const Split sp = find_split<SEL>(A, lane, 0, si);
-    if (sp.count == 1)
-        return;
-    const size_t hr = (size_t)sv.row * A.n_head + h;
-    if (sp.count == 0) {
-        const float z = sv.bad ? NAN : 0.0f;
-        if (tid < kMLanes && col < hd)
+    const size_t hr = (size_t)(A.row ? A.row[si] : si) * A.n_head + h;
+    if (count == 0) {
+        const float z = A.len[si] > A.max_pages << A.page_log ? NAN : 0.0f;
+        if (tid < LANES && col < hd)
             *(f4 *)(A.out + hr * hd + col) = f4{z, z, z, z};
         return;
     }
@@ -631,14 +800,14 @@ template <bool SEL, int ROWS> __global__ __launch_bounds__(256) void pages_merge
     const uint32_t at = col < hd ? col : 0;
     float m = -INFINITY, l = 0.0f;
     f4 a{0, 0, 0, 0};
-    for (uint32_t i0 = tid / kMLanes; i0 < sp.count; i0 += kMGroups * kMBatch) {
+    for (uint32_t i0 = tid / LANES; i0 < count; i0 += GROUPS * kMBatch) {
         float2 ml[kMBatch];
         f4 x[kMBatch];
 #pragma unroll
         for (int b = 0; b < kMBatch; b++) {
-            uint32_t i = i0 + kMGroups * b;
-            i = i < sp.count ? i : sp.count - 1;
-            const size_t pr = ((size_t)(sp.index + i) * tiles + tile) * ROWS + r % ROWS;
+            uint32_t i = i0 + GROUPS * b;
+            i = i < count ? i : count - 1;
+            const size_t pr = ((size_t)(first + i) * tiles + tile) * ROWS + r % ROWS;
             ml[b] = *(const float2 *)(A.part_ml + 2 * pr);
             x[b] = *(const f4 *)(A.part_acc + pr * hd + at);
         }
@@ -652,7 +821,7 @@ template <bool SEL, int ROWS> __global__ __launch_bounds__(256) void pages_merge
         m = mn;
 #pragma unroll
         for (int b = 0; b < kMBatch; b++) {
-            const bool in = i0 + kMGroups * b < sp.count && ml[b].x != -INFINITY;
+            const bool in = i0 + GROUPS * b < count && ml[b].x != -INFINITY;
             const float e = in ? __builtin_amdgcn_exp2f(ml[b].x - mn) : 0.0f;
             l += in ? e * ml[b].y : 0.0f;
 #pragma unroll
@@ -660,16 +829,16 @@ template <bool SEL, int ROWS> __global__ __launch_bounds__(256) void pages_merge
                 a[c] = __builtin_fmaf(e, x[b][c], a[c]);
         }
     }
-    /* the wave's 8 groups, then the 4 waves */
+    /* the wave's groups, then the 4 waves */
     float mw = m;
 #pragma unroll
-    for (int o = 8; o < 64; o <<= 1)
+    for (int o = LANES; o < 64; o <<= 1)
         mw = fmaxf(mw, __shfl_xor(mw, o, 64));
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mw);
     l *= f;
     a *= f;
 #pragma unroll
-    for (int o = 8; o < 64; o <<= 1) {
+    for (int o = LANES; o < 64; o <<= 1) {
         l += __shfl_xor(l, o, 64);
 #pragma unroll
         for (int c = 0; c < 4; c++)
@@ -679,10 +848,10 @@ template <bool SEL, int ROWS> __global__ __launch_bounds__(256) void pages_merge
         sM[w] = mw;
         sL[w] = l;
     }
-    if (lane < kMLanes)
+    if (lane < LANES)
         sA[w][lane] = a;
     __syncthreads();
-    if (tid >= kMLanes || col >= hd)
+    if (tid >= LANES || col >= hd)
         return;
     const float mx = fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3]));
     float sum = 0.0f;
@@ -711,9 +880,9 @@ template <bool SEL, int ROWS> __global__ __launch_bounds__(256) void pages_merge
 template <int T, int D> hipError_t launch_sel(const PagesArgs &a, hipStream_t s)
 {
     if (a.sel)
-        hipLaunchKernelGGL((pages_kernel<T, D, true>), dim3(a.n_wg), dim3(kPW * 64), 0, s, a);
+        hipLaunchKernelGGL((pages_kernel<T, D, true>), dim3(a.n_wg + 1), dim3(kPW * 64), 0, s, a);
     else
-        hipLaunchKernelGGL((pages_kernel<T, D, false>), dim3(a.n_wg), dim3(kPW * 64), 0, s, a);
+        hipLaunchKernelGGL((pages_kernel<T, D, false>), dim3(a.n_wg + 1), dim3(kPW * 64), 0, s, a);
     return hipGetLastError();
 }
 
@@ -740,10 +909,16 @@ int pages_supported(int kv, uint32_t hd)
            hd <= (kv == kF32 ? 256u : 512u);
 }
 
-uint32_t pages_share(uint32_t cus, uint32_t tiles)
+uint32_t pages_share(int kv, uint32_t hd, uint32_t cus, uint32_t tiles)
 {
-    const uint32_t fill = 4 * cus;
+    const uint32_t fill = pages_waves(kv, (int)hd) * cus;
     return fill / tiles > 1 ? fill / tiles : 1;
+}
+
+uint64_t pages_runs(uint32_t share, uint32_t n_seqs, uint64_t most_units)
+{
+    /* no more than the lengths that the table's rows hold can fill */
+    return std::min<uint64_t>(share, n_seqs * ((most_units + kLeastUnits - 1) / kLeastUnits));
 }
 
 hipError_t launch_pages(int kv, const PagesArgs &a, hipStream_t s)
@@ -761,18 +936,23 @@ hipError_t launch_pages(int kv, const PagesArgs &a, hipStream_t s)
     return hipErrorInvalidValue;
 }
 
+uint32_t pages_merge_cols(uint32_t n_seqs, uint32_t n_head, uint32_t hd)
+{
+    return hd > 32 && (uint64_t)n_seqs * n_head * ((hd + 127) / 128) >= kMergeFill ? 128 : 32;
+}
+
 hipError_t launch_pages_merge(int kv, const PagesArgs &a, hipStream_t s)
 {
-    const uint32_t n_wg = a.n_seqs * a.n_head * ((a.hd + kMCols - 1) / kMCols);
-    const bool f32 = kv == kF32;
-    if (a.sel && f32)
-        hipLaunchKernelGGL((pages_merge_kernel<true, 16>), dim3(n_wg), dim3(256), 0, s, a);
-    else if (a.sel)
-        hipLaunchKernelGGL((pages_merge_kernel<true, 8>), dim3(n_wg), dim3(256), 0, s, a);
-    else if (f32)
-        hipLaunchKernelGGL((pages_merge_kernel<false, 16>), dim3(n_wg), dim3(256), 0, s, a);
+    const uint32_t cols = pages_merge_cols(a.n_seqs, a.n_head, a.hd);
+    const uint32_t n_wg = a.n_seqs * a.n_head * ((a.hd + cols - 1) / cols);
+    if (kv == kF32 && cols == 128)
+        hipLaunchKernelGGL((pages_merge_kernel<16, 128>), dim3(n_wg), dim3(256), 0, s, a);
+    else if (kv == kF32)
+        hipLaunchKernelGGL((pages_merge_kernel<16, 32>), dim3(n_wg), dim3(256), 0, s, a);
+    else if (cols == 128)
+        hipLaunchKernelGGL((pages_merge_kernel<8, 128>), dim3(n_wg), dim3(256), 0, s, a);
     else
-        hipLaunchKernelGGL((pages_merge_kernel<false, 8>), dim3(n_wg), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((pages_merge_kernel<8, 32>), dim3(n_wg), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

@@ -109,10 +109,10 @@ int check_rows(const PagesGeom &g, const janas_attn_pages_call *c)
     return width > 0xFFFFFFFFu ? JANAS_ATTN_ERANGE : JANAS_ATTN_OK;
 }
 
-/* the splits of a call and the bytes of their partials */
+/* the runs of a call and the bytes of their partials */
 struct Parts {
     uint32_t rtiles, share;
-    uint64_t n_wg, ml_bytes, bytes;
+    uint64_t n_wg, plan_bytes, ml_bytes, bytes;
 };
 Parts parts_of(const PagesGeom &g, const janas_attn_pages *p)
 {
@@ -120,10 +120,13 @@ Parts parts_of(const PagesGeom &g, const janas_attn_pages *p)
     const uint32_t rows = pages_rows_wg(p->kv_type);
     t.rtiles = (g.group + rows - 1) / rows;
     const uint32_t tiles = g.n_kv * t.rtiles;
-    t.share = pages_share(g.cus, tiles);
-    t.n_wg = ((uint64_t)t.share + p->n_seqs) * tiles;
-    t.ml_bytes = (t.n_wg * rows * 2 * sizeof(float) + 255) / 256 * 256;
-    t.bytes = t.ml_bytes + t.n_wg * rows * g.hd * sizeof(float);
+    t.share = pages_share(p->kv_type, g.hd, g.cus, tiles);
+    const uint64_t runs = pages_runs(t.share, p->n_seqs, (uint64_t)p->max_pages * p->page / 16);
+    const uint64_t parts = (runs + p->n_seqs) * tiles * rows;
+    t.n_wg = runs * tiles;
+    t.plan_bytes = ((uint64_t)p->n_seqs * sizeof(uint2) + 255) / 256 * 256;
+    t.ml_bytes = (parts * 2 * sizeof(float) + 255) / 256 * 256;
+    t.bytes = t.plan_bytes + t.ml_bytes + parts * g.hd * sizeof(float);
     return t;
 }
 
@@ -292,10 +295,11 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
         (c->out_q8k && (uint64_t)g.n_head * g.hd % JANAS_ATTN_QK))
         return JANAS_ATTN_EINVAL;
     const Parts t = parts_of(g, p);
-    const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + 31) / 32);
+    const uint64_t cols = pages_merge_cols(p->n_seqs, g.n_head, g.hd);
+    const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + cols - 1) / cols);
     const uint64_t rows = c->row ? c->n_rows : p->n_seqs;
     const uint64_t blocks = rows * g.n_head * g.hd / JANAS_ATTN_QK;
-    if (std::max({t.n_wg, merge_wg, c->out_q8k ? blocks : 0}) > kMostThreads / 256)
+    if (std::max({t.n_wg + 1, merge_wg, c->out_q8k ? blocks : 0}) > kMostThreads / 256)
         return JANAS_ATTN_ERANGE;
     if (c->work_bytes < t.bytes)
         return JANAS_ATTN_ERANGE;
@@ -313,8 +317,9 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
     s.q = c->q;
     s.gate = c->gate;
     s.out = c->out;
-    s.part_ml = (float *)c->work;
-    s.part_acc = (float *)((char *)c->work + t.ml_bytes);
+    s.plan = (uint2 *)c->work;
+    s.part_ml = (float *)((char *)c->work + t.plan_bytes);
+    s.part_acc = (float *)((char *)c->work + t.plan_bytes + t.ml_bytes);
     s.n_seqs = p->n_seqs;
     s.n_rows = c->n_rows;
     s.max_pages = p->max_pages;
