@@ -347,24 +347,18 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         const uint32_t nb = (sv.end + page - 1) >> A.page_log;
         const uint32_t *const trow = A.table + (size_t)si * A.max_pages;
         const uint32_t *const srow = SEL ? A.sel + ((size_t)si * A.n_kv + kvh) * A.n_sel : nullptr;
-        uint32_t e0 = first >> upp_log, pid = 0, blk = 0;
+        uint32_t e0, pid = 0, blk = 0;
         bool bad = false;            /* a page outside the pool */
         auto fetch = [&](uint32_t from) {
-            const uint32_t e = from + lane;
-            const bool mine = e <= (last - 1) >> upp_log;
-            blk = mine ? e : kNone;
-            if constexpr (SEL) {
-                if (mine)
-                    blk = srow[e];
-            }
-            pid = 0;
-            if (blk < nb) {
-                pid = trow[blk];
-                bad |= pid >= A.n_pages;
-                pid = pid < A.n_pages ? pid : 0;
-            } else {
-                blk = kNone;
-            }
+            /* (entries behind the run's last one: that one again) */
+            const uint32_t lim = ((last > first ? last : su + u0) - 1) >> upp_log;
+            const uint32_t e = from + lane < lim ? from + lane : lim;
+            blk = SEL ? srow[e] : e;
+            const bool in = blk < nb;
+            pid = trow[in ? blk : 0];
+            bad |= in && pid >= A.n_pages;
+            pid = in && pid < A.n_pages ? pid : 0;
+            blk = in ? blk : kNone;
         };
 
         /* a unit: its page and KV head's rows, its first row and position (past
@@ -437,105 +431,88 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         };
 
         /* ---- the query: MFMA column n's (row n / 2, plane n & 1; f32: row n) as the
-           B operand of each K load, in registers or LDS. Planes: scaled by 2^ex so
-           that the row's largest lies in [2^13, 2^14) ---- */
+           B operand of each K load, in registers or LDS. Planes: scaled by 2^ex
+           so that the row's largest lies in [2^13, 2^14). Asked for first, made
+           when the first unit has been asked for: one round trip for the query
+           and the table, one for the unit ---- */
         constexpr int QN = 16 / EB;      /* numbers of a K load: 16, 8 or 4 */
         constexpr bool QLDS = S::QLDS;
+        /* LDS: the workgroup's rows once, 256 / ROWS lanes a row, words of four */
+        constexpr int TPR = kPW * 64 / ROWS, NQ = QLDS ? D / (4 * TPR) : KL * QN / 4;
+        const uint32_t qrow = QLDS ? tid / TPR : F32 ? n : n >> 1;
+        const float *const qsrc =
+            A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0 + (qrow < rows ? qrow : 0)) * hd;
+        f4 qx[NQ];
+        uint32_t qc[NQ];
+#pragma unroll
+        for (int j = 0; j < NQ; j++) {
+            qc[j] = QLDS ? 4 * (tid % TPR + TPR * j)
+                         : QN * (4 * (j / (QN / 4)) + g) + 4 * (j % (QN / 4));
+            qx[j] = *(const f4 *)(qsrc + (qc[j] < hd ? qc[j] : 0));
+        }
+        /* (a wave without units asks for a whole one all the same: no branch
+           holds up what follows) */
+        const uint32_t some = first < su + u0 ? first : su + u0 - 1;
+        e0 = some >> upp_log;
+        fetch(e0);
+        Unit x = unit_of(some);
+        load_k(x);
+        load_v(x);
+
         u4 qr[QLDS ? 1 : KL][QLDS ? 1 : EB == 1 ? 2 : 1];
-        float qs2;
-        auto plane_scale = [](float mx, int &ex) {
-            ex = 0;
-            if (mx > 0.0f && mx < INFINITY) {
-                frexpf(mx, &ex);
-                ex = 14 - ex;
-            }
-            return ldexpf(1.0f, ex);
-        };
-        if constexpr (QLDS) {
-            /* the workgroup's rows once: 256 / ROWS lanes a row, words of four */
-            constexpr int TPR = kPW * 64 / ROWS, NQ = D / (4 * TPR);
-            const uint32_t r = tid / TPR, t = tid % TPR;
-            const bool ok = r < rows;
-            const float *const src =
-                A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0 + (ok ? r : 0)) * hd;
-            f4 x[NQ];
-            float mx = 0.0f;
+        float qs2 = 1.0f, qmax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NQ; j++) {
+            if (qrow >= rows || qc[j] >= hd)
+                qx[j] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                qmax = fmaxf(qmax, fabsf(qx[j][e]));
+        }
+        if constexpr (F32) {
 #pragma unroll
             for (int j = 0; j < NQ; j++) {
-                const uint32_t c = 4 * (t + TPR * j);
-                x[j] = *(const f4 *)(src + (c < hd ? c : 0));
-                if (!ok || c >= hd)
-                    x[j] = f4{0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    mx = fmaxf(mx, fabsf(x[j][e]));
+                if constexpr (QLDS)
+                    *(f4 *)&sQ[qrow][qc[j]] = qx[j];
+                else
+                    qr[j][0] = __builtin_bit_cast(u4, qx[j]);
             }
-            if constexpr (F32) {
-#pragma unroll
-                for (int j = 0; j < NQ; j++)
-                    *(f4 *)&sQ[r][4 * (t + TPR * j)] = x[j];
-            } else {
-                mx = max_x16(max_row16(mx));
-                int ex;
-                const float up = plane_scale(mx, ex);
-#pragma unroll
-                for (int j = 0; j < NQ; j++) {
-                    h4 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        _Float16 a, b;
-                        split_hl(x[j][e] * up, a, b);
-                        hi[e] = a;
-                        lo[e] = b;
-                    }
-                    *(h4 *)&sQ[2 * r][2 * (t + TPR * j)] = hi;
-                    *(h4 *)&sQ[2 * r + 1][2 * (t + TPR * j)] = lo;
-                }
-                if (t == 0)
-                    sQs[r] = ldexpf(1.0f, -ex);
-            }
-            __syncthreads();
-            qs2 = F32 ? 1.0f : sQs[n >> 1];
         } else {
-            const uint32_t qrow = F32 ? n : n >> 1;
-            const bool ok = qrow < rows;
-            const float *const src =
-                A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0 + (ok ? qrow : 0)) * hd;
-            f4 x[KL][QN / 4];
-            float mx = 0.0f;
-#pragma unroll
-            for (int i = 0; i < KL; i++)
-#pragma unroll
-                for (int j = 0; j < QN / 4; j++) {
-                    const uint32_t c = QN * (4 * i + g) + 4 * j;
-                    x[i][j] = *(const f4 *)(src + (c < hd ? c : 0));
-                    if (!ok || c >= hd)
-                        x[i][j] = f4{0, 0, 0, 0};
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        mx = fmaxf(mx, fabsf(x[i][j][e]));
-                }
+            /* the row's lanes: 32 side by side, or the four with the same n */
+            qmax = QLDS ? max_x16(max_row16(qmax)) : max_x32(max_x16(qmax));
             int ex = 0;
-            const float up = plane_scale(max_x32(max_x16(mx)), ex);
+            if (qmax > 0.0f && qmax < INFINITY) {
+                frexpf(qmax, &ex);
+                ex = 14 - ex;
+            }
+            const float up = ldexpf(1.0f, ex);
+            qs2 = ldexpf(1.0f, -ex);
 #pragma unroll
-            for (int i = 0; i < KL; i++) {
-                if constexpr (F32) {
-                    qr[i][0] = __builtin_bit_cast(u4, x[i][0]);
+            for (int j = 0; j < NQ; j++) {
+                h4 hi, lo;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    _Float16 y, z;
+                    split_hl(qx[j][e] * up, y, z);
+                    hi[e] = y;
+                    lo[e] = z;
+                }
+                if constexpr (QLDS) {
+                    *(h4 *)&sQ[2 * qrow][qc[j] / 2] = hi;
+                    *(h4 *)&sQ[2 * qrow + 1][qc[j] / 2] = lo;
                 } else {
-#pragma unroll
-                    for (int j = 0; j < QN / 8; j++) {
-                        h8 y;
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            _Float16 hi, lo;
-                            split_hl(x[i][2 * j + e / 4][e & 3] * up, hi, lo);
-                            y[e] = n & 1 ? lo : hi;
-                        }
-                        qr[i][j] = __builtin_bit_cast(u4, y);
-                    }
+                    const uint2 y = __builtin_bit_cast(uint2, n & 1 ? lo : hi);
+                    qr[j / (QN / 4)][j % (QN / 4) / 2][2 * (j & 1)] = y.x;
+                    qr[j / (QN / 4)][j % (QN / 4) / 2][2 * (j & 1) + 1] = y.y;
                 }
             }
-            qs2 = F32 ? 1.0f : ldexpf(1.0f, -ex);
+            if (QLDS && tid % TPR == 0)
+                sQs[qrow] = qs2;
+        }
+        if constexpr (QLDS) {
+            __syncthreads();
+            if constexpr (!F32)
+                qs2 = sQs[n >> 1];
         }
         qs2 = qs2 * A.scale * kLog2e;
         /* operand j of K load i; `at`: the lane's place in LDS, unknown to the
@@ -558,132 +535,126 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                                            within */
         float vup = 0.0f;               /* a weight's factor: 2^kUp over theirs */
         const float keep = lane & 1 ? -1.0f : -0.0f;
-        if (first < last) {
-            fetch(e0);
-            Unit x = unit_of(first);
-            load_k(x);
-            load_v(x);
-            for (uint32_t u = first; u < last; u++) {
-                const Unit now = x;
-                const bool more = u + 1 < last;
-                if (more)
-                    x = unit_of(u + 1);
-                /* scores: lane holds positions 4 g + j of MFMA column n */
-                f4 s{0, 0, 0, 0};
-                uint32_t place = n * S::QROW * 4 + 16 * (EB == 1 ? 2 : 1) * g;
-                if constexpr (QLDS)
-                    asm volatile("" : "+v"(place));
+        for (uint32_t u = first; u < last; u++) {
+            const Unit now = x;
+            const bool more = u + 1 < last;
+            if (more)
+                x = unit_of(u + 1);
+            /* scores: lane holds positions 4 g + j of MFMA column n */
+            f4 s{0, 0, 0, 0};
+            uint32_t place = n * S::QROW * 4 + 16 * (EB == 1 ? 2 : 1) * g;
+            if constexpr (QLDS)
+                asm volatile("" : "+v"(place));
 #pragma unroll
-                for (int i = 0; i < KL; i++) {
-                    const u4 q0 = q_operand(i, 0, place);
-                    if constexpr (F32) {
-                        const f4 kf = __builtin_bit_cast(f4, kr[i]), qf = __builtin_bit_cast(f4, q0);
+            for (int i = 0; i < KL; i++) {
+                const u4 q0 = q_operand(i, 0, place);
+                if constexpr (F32) {
+                    const f4 kf = __builtin_bit_cast(f4, kr[i]), qf = __builtin_bit_cast(f4, q0);
 #pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s, 0, 0, 0);
-                    } else if constexpr (T == kI8) {
-                        const u4 y = unit_fix(kr[i], kback[i]);
-                        s = mfma(i8_widen8(y.x, y.y), __builtin_bit_cast(h8, q0), s);
-                        s = mfma(i8_widen8(y.z, y.w), __builtin_bit_cast(h8, q_operand(i, 1, place)), s);
-                    } else if constexpr (T == kI16) {
-                        h8 hi, lo;
-                        i16_planes8(kr[i].x, kr[i].y, kr[i].z, kr[i].w, hi, lo);
-                        s = mfma(hi, __builtin_bit_cast(h8, q0), s);
-                        s = mfma(lo, __builtin_bit_cast(h8, q0), s);
-                    } else {
-                        s = mfma(__builtin_bit_cast(h8, kr[i]), __builtin_bit_cast(h8, q0), s);
-                    }
+                    for (int e = 0; e < 4; e++)
+                        s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s, 0, 0, 0);
+                } else if constexpr (T == kI8) {
+                    const u4 y = unit_fix(kr[i], kback[i]);
+                    s = mfma(i8_widen8(y.x, y.y), __builtin_bit_cast(h8, q0), s);
+                    s = mfma(i8_widen8(y.z, y.w), __builtin_bit_cast(h8, q_operand(i, 1, place)), s);
+                } else if constexpr (T == kI16) {
+                    h8 hi, lo;
+                    i16_planes8(kr[i].x, kr[i].y, kr[i].z, kr[i].w, hi, lo);
+                    s = mfma(hi, __builtin_bit_cast(h8, q0), s);
+                    s = mfma(lo, __builtin_bit_cast(h8, q0), s);
+                } else {
+                    s = mfma(__builtin_bit_cast(h8, kr[i]), __builtin_bit_cast(h8, q0), s);
                 }
-                const f4 kz = ks;
-                if (more)
-                    load_k(x);
-                if (now.pos < sv.end && now.pos + kUnit > sv.lo) {
-                    f4 vz = vs;
+            }
+            const f4 kz = ks;
+            if (more)
+                load_k(x);
+            if (now.pos < sv.end && now.pos + kUnit > sv.lo) {
+                f4 vz = vs;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (!F32)
+                        s[j] += from_x1(s[j]);
+                    s[j] *= qs2;
+                    if constexpr (SCALED)
+                        s[j] *= kz[j];
+                }
+                if (now.pos < sv.lo || now.pos + kUnit > sv.end) {
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        if constexpr (!F32)
-                            s[j] += from_x1(s[j]);
-                        s[j] *= qs2;
-                        if constexpr (SCALED)
-                            s[j] *= kz[j];
+                        const uint32_t p = now.pos + 4 * g + j;
+                        const bool in = p >= sv.lo && p < sv.end;
+                        s[j] = in ? s[j] : -INFINITY;
+                        vz[j] = in ? vz[j] : 0.0f;
                     }
-                    if (now.pos < sv.lo || now.pos + kUnit > sv.end) {
+                }
+                const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+                uint32_t ex = 0;
+                if constexpr (SCALED)
+                    ex = exponent(fmaxf(fmaxf(vz[0], vz[1]), fmaxf(vz[2], vz[3])));
+                if (__any(top > m + kLazy || ex > ev)) {
+                    /* new references; what is summed so far follows */
+                    const float mn = fmaxf(m, max_x32(max_x16(top)));
+                    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
+                    l *= f;
+                    float fe = 1.0f;
+                    if constexpr (SCALED) {
+                        const uint32_t en = (uint32_t)fmaxf((float)ev, max_x32(max_x16((float)ex)));
+                        fe = ldexpf(1.0f, (int)ev - (int)en);
+                        ev = en;
+                    }
+                    vup = ldexpf(1.0f, kUp + (SCALED ? 126 - (int)ev : 0));
+                    float fr[4];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const uint32_t p = now.pos + 4 * g + j;
-                            const bool in = p >= sv.lo && p < sv.end;
-                            s[j] = in ? s[j] : -INFINITY;
-                            vz[j] = in ? vz[j] : 0.0f;
-                        }
-                    }
-                    const float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
-                    uint32_t ex = 0;
-                    if constexpr (SCALED)
-                        ex = exponent(fmaxf(fmaxf(vz[0], vz[1]), fmaxf(vz[2], vz[3])));
-                    if (__any(top > m + kLazy || ex > ev)) {
-                        /* new references; what is summed so far follows */
-                        const float mn = fmaxf(m, max_x32(max_x16(top)));
-                        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-                        m = mn;
-                        l *= f;
-                        float fe = 1.0f;
-                        if constexpr (SCALED) {
-                            const uint32_t en = (uint32_t)fmaxf((float)ev, max_x32(max_x16((float)ex)));
-                            fe = ldexpf(1.0f, (int)ev - (int)en);
-                            ev = en;
-                        }
-                        vup = ldexpf(1.0f, kUp + (SCALED ? 126 - (int)ev : 0));
-                        float fr[4];
+                    for (int i = 0; i < 4; i++)
+                        fr[i] = __shfl(f, (int)(4 * g + (F32 ? i : i & 2)), 64) * fe;
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
 #pragma unroll
                         for (int i = 0; i < 4; i++)
-                            fr[i] = __shfl(f, (int)(4 * g + (F32 ? i : i & 2)), 64) * fe;
-#pragma unroll
-                        for (int t = 0; t < NT; t++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++)
-                                o[t][i] *= fr[i];
-                    }
-                    const float mm = m == -INFINITY ? 0.0f : m;
-                    h4 pa;
-                    f4 pf;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float p = __builtin_amdgcn_exp2f(s[j] - mm);
-                        l += p;
-                        pf[j] = p;
-                        if constexpr (!F32) {
-                            float pv = p * vup;
-                            if constexpr (SCALED)
-                                pv *= vz[j];
-                            asm volatile("" : "+v"(pv));
-                            const float hi = (float)(_Float16)pv;
-                            pa[j] = (_Float16)__builtin_fmaf(keep, hi, pv);
-                        }
-                    }
-                    /* values: product e of a unit of columns */
-#pragma unroll
-                    for (int c = 0; c < VU; c++)
-#pragma unroll
-                        for (int e = 0; e < VN; e++) {
-                            const int t = c * VN + e;
-                            if constexpr (F32) {
-#pragma unroll
-                                for (int j = 0; j < 4; j++)
-                                    o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                        pf[j], __uint_as_float(word<VW>(vr[j][c], e)), o[t], 0, 0, 0);
-                            } else {
-                                const VT v4[4] = {vr[0][c], vr[1][c], vr[2][c], vr[3][c]};
-                                h4 vb[DP];
-                                value_operand<T, VW>(v4, e, vb);
-#pragma unroll
-                                for (int d = 0; d < DP; d++)
-                                    o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, vb[d], o[t], 0, 0, 0);
-                            }
-                        }
+                            o[t][i] *= fr[i];
                 }
-                if (more)
-                    load_v(x);
+                const float mm = m == -INFINITY ? 0.0f : m;
+                h4 pa;
+                f4 pf;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float p = __builtin_amdgcn_exp2f(s[j] - mm);
+                    l += p;
+                    pf[j] = p;
+                    if constexpr (!F32) {
+                        float pv = p * vup;
+                        if constexpr (SCALED)
+                            pv *= vz[j];
+                        asm volatile("" : "+v"(pv));
+                        const float hi = (float)(_Float16)pv;
+                        pa[j] = (_Float16)__builtin_fmaf(keep, hi, pv);
+                    }
+                }
+                /* values: product e of a unit of columns */
+#pragma unroll
+                for (int c = 0; c < VU; c++)
+#pragma unroll
+                    for (int e = 0; e < VN; e++) {
+                        const int t = c * VN + e;
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                                    pf[j], __uint_as_float(word<VW>(vr[j][c], e)), o[t], 0, 0, 0);
+                        } else {
+                            const VT v4[4] = {vr[0][c], vr[1][c], vr[2][c], vr[3][c]};
+                            h4 vb[DP];
+                            value_operand<T, VW>(v4, e, vb);
+#pragma unroll
+                            for (int d = 0; d < DP; d++)
+                                o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, vb[d], o[t], 0, 0, 0);
+                        }
+                    }
             }
+            if (more)
+                load_v(x);
         }
 
         /* ---- the waves joined ---- */

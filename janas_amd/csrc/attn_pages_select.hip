@@ -149,74 +149,288 @@ __device__ __forceinline__ Blocks blocks_in_sight(const SelectArgs &A, const Seq
     return Blocks{b0, ((s.end + page - 1) >> A.page_log) - b0};
 }
 
+template <int CTRL> __device__ __forceinline__ double dpp(double x)
+{
+    const uint2 u = __builtin_bit_cast(uint2, x);
+    return __builtin_bit_cast(
+        double, make_uint2(__builtin_amdgcn_update_dpp(0u, u.x, CTRL, 0xf, 0xf, false),
+                           __builtin_amdgcn_update_dpp(0u, u.y, CTRL, 0xf, 0xf, false)));
+}
+/* over 16 lanes: quad_perm [1, 0, 3, 2], [2, 3, 0, 1], row_ror 8 and 4 */
 __device__ __forceinline__ double sum16(double x)
 {
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1)
-        x += __shfl_xor(x, o, 64);
-    return x;
+    x += dpp<0xB1>(x);
+    x += dpp<0x4E>(x);
+    x += dpp<0x128>(x);
+    return x + dpp<0x124>(x);
 }
 
 constexpr uint32_t kScoreBlocks = 16;  /* blocks a workgroup at once, 16 lanes each */
 
-__global__ __launch_bounds__(256) void score_kernel(const SelectArgs A)
+/*
+ * A block's 16 lanes take 8 dimensions of every 128 each; HC: 128s of the head
+ * size. The query of 4 / HC heads stays in registers, as doubles and as the mask
+ * of its positive numbers, while the lanes go from block to block, the next
+ * block's bounds asked for before this one's are used: a number and head are a
+ * bit select, a conversion and a multiply-add. A group of more heads goes over
+ * the blocks again.
+ */
+template <int HC> __global__ __launch_bounds__(256) void score_kernel(const SelectArgs A)
 {
+    constexpr uint32_t HT = 4 / HC;
     const uint32_t tid = threadIdx.x, si = blockIdx.z, kvh = blockIdx.y;
     const SeqView sv = seq_view(A, si);
     const Blocks bl = blocks_in_sight(A, sv);
     if (bl.n <= A.n_sel)
         return; /* all of them */
-    const uint32_t c = tid % 16, hd = A.hd;
-    const float *const q = A.q + (size_t)sv.row * A.q_stride + (size_t)kvh * A.group * hd;
+    const uint32_t c = tid % 16, hd = A.hd, step = gridDim.x * kScoreBlocks;
+    const uint32_t j0 = blockIdx.x * kScoreBlocks + tid / 16;
+    if (j0 >= bl.n)
+        return; /* (a row of 16 lanes is whole or not there) */
+    const uint32_t *const table = A.table + (size_t)si * A.max_pages + bl.b0;
     float *const out = A.score + ((size_t)si * A.n_kv + kvh) * A.max_pages;
-    for (uint32_t j = blockIdx.x * kScoreBlocks + tid / 16; j < bl.n; j += gridDim.x * kScoreBlocks) {
-        uint32_t pid = A.table[(size_t)si * A.max_pages + bl.b0 + j];
+    bool in[HC];
+#pragma unroll
+    for (int i = 0; i < HC; i++)
+        in[i] = 128 * i + 8 * c < hd;
+    auto boxes = [&](uint32_t j, h8 *lo, h8 *hi) {
+        uint32_t pid = table[j];
         pid = pid < A.n_pages ? pid : 0;
         const _Float16 *const box = A.bounds + ((size_t)pid * A.n_kv + kvh) * 2 * hd;
-        float best = -INFINITY;
-        for (uint32_t h = 0; h < A.group; h++) {
-            double s = 0.0;
-            for (uint32_t d = 8 * c; d < hd; d += 128) {
-                const h8 lo = *(const h8 *)(box + d), hi = *(const h8 *)(box + hd + d);
-                const float *const qd = q + (size_t)h * hd + d;
-                const f4 qa = *(const f4 *)qd, qc = *(const f4 *)(qd + 4);
+#pragma unroll
+        for (int i = 0; i < HC; i++) {
+            const uint32_t d = in[i] ? 128 * i + 8 * c : 0;
+            lo[i] = *(const h8 *)(box + d);
+            hi[i] = *(const h8 *)(box + hd + d);
+        }
+    };
+    for (uint32_t h0 = 0; h0 < A.group; h0 += HT) {
+        const float *const q =
+            A.q + (size_t)sv.row * A.q_stride + ((size_t)kvh * A.group + h0) * hd;
+        double x[HT][HC][8];
+        uint32_t m[HT][HC][8];
+#pragma unroll
+        for (uint32_t h = 0; h < HT; h++)
+#pragma unroll
+            for (int i = 0; i < HC; i++) {
+                const bool ok = in[i] && h0 + h < A.group;
+                const float *const p = q + (ok ? (size_t)h * hd + 128 * i + 8 * c : 0);
+                const f4 a = *(const f4 *)p, b = *(const f4 *)(p + 4);
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    float x = e < 4 ? qa[e & 3] : qc[e & 3];
-                    x = A.negate ? -x : x;
-                    const float b = (float)(x > 0.0f ? hi[e] : lo[e]);
-                    s = __builtin_fma((double)x, (double)b, s);
+                    float y = e < 4 ? a[e & 3] : b[e & 3];
+                    y = !ok ? 0.0f : A.negate ? -y : y;
+                    x[h][i][e] = (double)y;
+                    m[h][i][e] = y > 0.0f ? 0xFFFFFFFFu : 0;
                 }
             }
-            best = fmaxf(best, (float)sum16(s));
+        h8 lo[HC], hi[HC];
+        boxes(j0, lo, hi);
+        for (uint32_t j = j0; j < bl.n; j += step) {
+            uint32_t l[HC][8], u[HC][8];
+#pragma unroll
+            for (int i = 0; i < HC; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    l[i][e] = __float_as_uint((float)lo[i][e]);
+                    u[i][e] = __float_as_uint((float)hi[i][e]);
+                }
+            if (j + step < bl.n)
+                boxes(j + step, lo, hi);
+            float best = -INFINITY;
+#pragma unroll
+            for (uint32_t h = 0; h < HT; h++) {
+                double s = 0.0;
+#pragma unroll
+                for (int i = 0; i < HC; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const uint32_t k = m[h][i][e];
+                        const float b = __uint_as_float((u[i][e] & k) | (l[i][e] & ~k));
+                        s = __builtin_fma(x[h][i][e], (double)b, s);
+                    }
+                const float y = (float)sum16(s);
+                if (h0 + h < A.group)
+                    best = fmaxf(best, y);
+            }
+            if (c == 0)
+                out[j] = h0 == 0 ? best : fmaxf(best, out[j]);
         }
-        if (c == 0)
-            out[j] = best;
     }
 }
 
 constexpr uint32_t kPickThreads = 1024;
 constexpr uint32_t kPickWaves = kPickThreads / 64;
+constexpr uint32_t kPickKeys = 8;      /* keys a thread keeps in registers */
 
-/* a score's place in order, as a whole number above 0 */
+/* a score's place in order, as a whole number */
 __device__ __forceinline__ uint32_t score_key(float x)
 {
     const uint32_t u = __float_as_uint(x + 0.0f); /* (-0 is 0) */
-    const uint32_t k = u & 0x80000000u ? ~u : u | 0x80000000u;
-    return k == 0 ? 1 : k == 0xFFFFFFFFu ? 0xFFFFFFFEu : k;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+/* the sum over the lanes up to and with this one (as scan_wave in
+   attn_pages.hip) */
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t shifted(uint32_t x)
+{
+    return __builtin_amdgcn_update_dpp(0u, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x)
+{
+    x += shifted<0x111, 0xf>(x);
+    x += shifted<0x112, 0xf>(x);
+    x += shifted<0x114, 0xf>(x);
+    x += shifted<0x118, 0xf>(x);
+    x += shifted<0x142, 0xa>(x);
+    x += shifted<0x143, 0xc>(x);
+    return x;
 }
 
 /*
- * One workgroup a (sequence, KV head). The n_sel-th largest key is found 8 bits
- * at a time from the top (a histogram of the keys that share the bits found so
- * far); then the blocks above it, and of those at it the lowest, are written in
- * order by a running count.
+ * One workgroup a (sequence, KV head). Of the blocks that are not forced, the
+ * `want`-th largest key is found 8 bits at a time, from the highest bit in which
+ * they differ at all, by a histogram of the keys that share the bits found so
+ * far; it is enough to know the bits above which exactly `want` keys lie. Then
+ * each thread counts its own chosen blocks - neighbours, so that a scan of the
+ * counts puts them in order - and writes them. REG: the thread's keys stay in
+ * registers; else they are read again at each step.
  */
-__global__ __launch_bounds__(kPickThreads) void pick_kernel(const SelectArgs A)
+template <bool REG> __device__ void pick(const SelectArgs &A, const Blocks &bl, const float *score,
+                                         uint32_t *sel)
 {
-    __shared__ uint32_t sHist[256], sFound[2];
+    __shared__ uint32_t sHist[4][256], sFound[4][3];
+    __shared__ uint32_t sLow[kPickWaves], sHigh[kPickWaves];
     __shared__ uint32_t sAbove[kPickWaves], sAt[kPickWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint32_t per = (bl.n + kPickThreads - 1) / kPickThreads, first = tid * per;
+    const uint32_t mine = first >= bl.n ? 0 : bl.n - first < per ? bl.n - first : per;
+    auto forced = [&](uint32_t j) { return j < A.first || j >= bl.n - A.last; };
+    uint32_t kept[REG ? kPickKeys : 1];
+    if constexpr (REG) {
+#pragma unroll
+        for (uint32_t r = 0; r < kPickKeys; r++)
+            if (r < mine)
+                kept[r] = score_key(score[first + r]);
+    }
+    /* f(j, key) for the thread's blocks that are not forced */
+    auto each = [&](auto f) {
+        if constexpr (REG) {
+#pragma unroll
+            for (uint32_t r = 0; r < kPickKeys; r++)
+                if (r < mine && !forced(first + r))
+                    f(first + r, kept[r]);
+        } else {
+            for (uint32_t r = 0; r < mine; r++)
+                if (!forced(first + r))
+                    f(first + r, score_key(score[first + r]));
+        }
+    };
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+    each([&](uint32_t, uint32_t k) {
+        low = k < low ? k : low;
+        high = k > high ? k : high;
+    });
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const uint32_t a = __shfl_xor(low, o, 64), b = __shfl_xor(high, o, 64);
+        low = a < low ? a : low;
+        high = b > high ? b : high;
+    }
+    if (lane == 0) {
+        sLow[w] = low;
+        sHigh[w] = high;
+    }
+    ((uint32_t *)sHist)[tid] = 0;
+    __syncthreads();
+    for (uint32_t i = 0; i < kPickWaves; i++) {
+        low = sLow[i] < low ? sLow[i] : low;
+        high = sHigh[i] > high ? sHigh[i] : high;
+    }
+    /* keys >= edge with the bits of `mask` are chosen, those equal to it in them
+       until `want` is used up */
+    uint32_t want = A.n_sel - A.first - A.last, bits = low == high ? 0 : 32 - __builtin_clz(low ^ high);
+    uint32_t mask = bits == 32 ? 0 : 0xFFFFFFFFu << bits, edge = high & mask;
+    for (int pass = 0; bits > 0 && want > 0; pass++) {
+        const uint32_t shift = bits > 8 ? bits - 8 : 0, digits = (1u << (bits - shift)) - 1;
+        each([&](uint32_t, uint32_t k) {
+            if ((k & mask) == edge)
+                atomicAdd(&sHist[pass][k >> shift & digits], 1u);
+        });
+        __syncthreads();
+        /* the bin of the want-th from the top: one wave, 4 bins a lane from the
+           top one down */
+        if (w == 0) {
+            uint32_t n[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                n[e] = sHist[pass][255 - (4 * lane + e)];
+                sum += n[e];
+            }
+            const uint32_t s = scan_wave(sum);
+            uint32_t before = s - sum;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (before < want && want <= before + n[e]) {
+                    sFound[pass][0] = 255 - (4 * lane + e);
+                    sFound[pass][1] = want - before;
+                    sFound[pass][2] = n[e];
+                }
+                before += n[e];
+            }
+        }
+        __syncthreads();
+        bits = shift;
+        mask |= digits << shift;
+        edge |= sFound[pass][0] << shift;
+        want = sFound[pass][1];
+        if (want == sFound[pass][2])
+            break; /* all of that bin */
+    }
+    uint32_t above = 0, at = 0;
+    each([&](uint32_t, uint32_t k) {
+        above += (k & mask) > edge;
+        at += (k & mask) == edge;
+    });
+    /* (the forced ones count as above) */
+    for (uint32_t r = 0; r < mine; r++)
+        above += forced(first + r);
+    const uint32_t sa = scan_wave(above), st = scan_wave(at);
+    if (lane == 63) {
+        sAbove[w] = sa;
+        sAt[w] = st;
+    }
+    __syncthreads();
+    uint32_t na = sa - above, nt = st - at;
+    for (uint32_t i = 0; i < kPickWaves; i++) {
+        na += i < w ? sAbove[i] : 0;
+        nt += i < w ? sAt[i] : 0;
+    }
+    auto put = [&](uint32_t j, bool over, bool equal) {
+        if (over || (equal && nt < want))
+            sel[na + (nt < want ? nt : want)] = bl.b0 + j;
+        na += over;
+        nt += equal;
+    };
+    if constexpr (REG) {
+#pragma unroll
+        for (uint32_t r = 0; r < kPickKeys; r++)
+            if (r < mine) {
+                const bool f = forced(first + r);
+                put(first + r, f || (kept[r] & mask) > edge, !f && (kept[r] & mask) == edge);
+            }
+    } else {
+        for (uint32_t r = 0; r < mine; r++) {
+            const bool f = forced(first + r);
+            const uint32_t k = f ? 0 : score_key(score[first + r]) & mask;
+            put(first + r, f || k > edge, !f && k == edge);
+        }
+    }
+}
+
+__global__ __launch_bounds__(kPickThreads) void pick_kernel(const SelectArgs A)
+{
+    const uint32_t tid = threadIdx.x;
     const uint32_t kvh = blockIdx.x % A.n_kv, si = blockIdx.x / A.n_kv;
     const SeqView sv = seq_view(A, si);
     if (!sv.part)
@@ -229,79 +443,10 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(const SelectArgs A)
         return;
     }
     const float *const score = A.score + ((size_t)si * A.n_kv + kvh) * A.max_pages;
-    /* the forced ones above every other */
-    auto key = [&](uint32_t j) {
-        return j < A.first || j >= bl.n - A.last ? 0xFFFFFFFFu : score_key(score[j]);
-    };
-    uint32_t found = 0, mask = 0, want = A.n_sel;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256)
-            sHist[tid] = 0;
-        __syncthreads();
-        for (uint32_t j = tid; j < bl.n; j += kPickThreads) {
-            const uint32_t k = key(j);
-            if ((k & mask) == found)
-                atomicAdd(&sHist[k >> shift & 255], 1u);
-        }
-        __syncthreads();
-        /* the bin that holds the want-th from the top: one wave, 4 bins a lane
-           from the top bin down */
-        if (w == 0) {
-            uint32_t n[4], sum = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                n[e] = sHist[255 - (4 * lane + e)];
-                sum += n[e];
-            }
-            uint32_t s = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t y = __shfl_up(s, o, 64);
-                s += lane >= (uint32_t)o ? y : 0;
-            }
-            uint32_t before = s - sum;
-            if (before < want && want <= s) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    if (before < want && want <= before + n[e]) {
-                        sFound[0] = 255 - (4 * lane + e);
-                        sFound[1] = want - before;
-                    }
-                    before += n[e];
-                }
-            }
-        }
-        __syncthreads();
-        found |= sFound[0] << shift;
-        want = sFound[1];
-        mask |= 255u << shift;
-        __syncthreads();
-    }
-    /* `found` is the n_sel-th key; `want` of those equal to it are taken */
-    uint32_t above = 0, at = 0; /* blocks above it and at it before this round */
-    for (uint32_t j0 = 0; j0 < bl.n; j0 += kPickThreads) {
-        const uint32_t j = j0 + tid;
-        const uint32_t k = j < bl.n ? key(j) : 0;
-        const uint64_t ma = __ballot(k > found), me = __ballot(k == found);
-        if (lane == 0) {
-            sAbove[w] = __popcll(ma);
-            sAt[w] = __popcll(me);
-        }
-        __syncthreads();
-        uint32_t na = above, ne = at;
-        for (uint32_t i = 0; i < kPickWaves; i++) {
-            na += i < w ? sAbove[i] : 0;
-            ne += i < w ? sAt[i] : 0;
-            above += sAbove[i];
-            at += sAt[i];
-        }
-        __syncthreads();
-        const uint64_t below = (1ull << lane) - 1;
-        na += __popcll(ma & below);
-        ne += __popcll(me & below);
-        if (k > found || (k == found && k && ne < want))
-            sel[na + (ne < want ? ne : want)] = bl.b0 + j;
-    }
+    if (bl.n <= kPickKeys * kPickThreads)
+        pick<true>(A, bl, score, sel);
+    else
+        pick<false>(A, bl, score, sel);
 }
 
 }  // namespace
@@ -320,7 +465,13 @@ hipError_t launch_select(const SelectArgs &a, hipStream_t s)
     uint32_t x = (a.max_pages + kScoreBlocks - 1) / kScoreBlocks;
     const uint32_t most = pairs < 8 * a.cus ? 8 * a.cus / pairs : 1;
     x = x < most ? x : most;
-    hipLaunchKernelGGL(score_kernel, dim3(x, a.n_kv, a.n_seqs), dim3(256), 0, s, a);
+    const dim3 grid(x, a.n_kv, a.n_seqs);
+    if (a.hd <= 128)
+        hipLaunchKernelGGL(score_kernel<1>, grid, dim3(256), 0, s, a);
+    else if (a.hd <= 256)
+        hipLaunchKernelGGL(score_kernel<2>, grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL(score_kernel<4>, grid, dim3(256), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess)
         return e;

@@ -551,14 +551,15 @@ def test_select(gpu, h, n_kv, hd, n_sel, first, last, window):
                 assert np.array_equal(want, got[i, kh]), (i, n, kh, want, got[i, kh])
 
 
-def test_select_ties_and_many_blocks(gpu):
+@pytest.mark.parametrize("nb", [1025, 2500, 8193])
+def test_select_ties_and_many_blocks(gpu, nb):
     """Blocks of equal scores (the lower is taken), all of them equal, scores of
-    both signs and zeros of both signs, over more blocks than threads."""
+    both signs and zeros of both signs, over more blocks than threads, and than
+    keys that stay in registers."""
     h, n_kv, hd, page = 2, 1, 64, 16
     rng = np.random.default_rng(6)
-    lens = [40000, 40000, 39999]
+    lens = [16 * nb, 16 * nb, 16 * nb - 1]
     pool = ph.Pool(rng, KV_I8, [16] * 3, page, n_kv, hd)
-    nb = 2500
     pool.n_pages = nb
     pool.k = np.zeros((nb, n_kv, page, hd), np.int8)
     pool.v, pool.ks = pool.k, np.zeros((nb, n_kv, page), np.float32)
@@ -571,7 +572,7 @@ def test_select_ties_and_many_blocks(gpu):
     q = np.zeros((3, h, hd), np.float32)
     q[:, 0, 0], q[:, 1, 0] = 1.0, -0.5
     q[1] = 0.0
-    for n_sel, first, last in ((900, 1, 3), (2499, 0, 0), (1, 0, 0), (60, 0, 0)):
+    for n_sel, first, last in ((900, 1, 3), (nb - 1, 0, 0), (1, 0, 0), (60, 0, 0), (7, 3, 4)):
         got, _ = selected(gpu, pool, h, q, n_sel, first, last, boxes=boxes)
         for i, n in enumerate(lens):
             want = ph.choose(q[i], boxes[pool.table[i]][:, 0], n, 0, page, n_sel, first, last)
