@@ -638,9 +638,9 @@ __global__ __launch_bounds__(256) void pages_rows16_kernel(const PagesRowArgs A)
         k[b] = v[b] = nw[b] = f4{0, 0, 0, 0};
         if (col >= hd)
             continue;
-        k[b] = *(const f4 *)(src + col);
+        k[b] = __builtin_nontemporal_load((const f4 *)(src + col));
         if (!query)
-            v[b] = *(const f4 *)(vsrc + col);
+            v[b] = __builtin_nontemporal_load((const f4 *)(vsrc + col));
         if (norm)
             nw[b] = *(const f4 *)(norm + col);
     }
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(256) void pages_rows16_kernel(const PagesRowArgs A)
 #pragma unroll
         for (int b = 0; b < NB; b++)
             if (64 * b + 4 * c < hd)
-                *(f4 *)(dst + 64 * b + 4 * c) = k[b];
+                __builtin_nontemporal_store(k[b], (f4 *)(dst + 64 * b + 4 * c));
         return;
     }
     if (A.v_norm) {

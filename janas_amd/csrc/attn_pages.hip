@@ -287,22 +287,27 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
     __shared__ RunsLds sR;
 
     const uint32_t thread = threadIdx.x, w = __builtin_amdgcn_readfirstlane(thread >> 6);
-    const uint32_t tiles = A.n_kv * A.rtiles, tile = blockIdx.x % tiles, run = blockIdx.x / tiles;
+    /* with more than 64 sequences, one workgroup more, the first, writes the plan;
+       else the first does it besides */
+    const bool planner = A.n_seqs > 64;
+    const uint32_t id = blockIdx.x - (planner ? 1 : 0);
+    const uint32_t tiles = A.n_kv * A.rtiles, tile = id % tiles, run = id / tiles;
     Runs<SEL> R;
     R.begin(A, thread & 63, w, sR);
-    if (blockIdx.x == A.n_wg) {
-        /* one workgroup more: for the merge, each sequence's partials - the one
-           of run x and sequence i has number x + i */
+    if (blockIdx.x == 0) {
+        /* for the merge, each sequence's partials: the one of run x and sequence
+           i has number x + i */
         const uint32_t lane = thread & 63;
         do {
             const uint32_t i = R.i0 + lane, u = sR.units[lane];
             const uint64_t r0 = sR.from[lane] / R.per;
             const uint64_t r1 = u ? (sR.from[lane] + u - 1) / R.per + 1 : r0;
-            if (w == 0 && i < A.n_seqs)
+            if (w == kPW - 1 && i < A.n_seqs)
                 A.plan[i] = make_uint2((uint32_t)r0 + i,
                                        sR.row[lane] == kNone ? kNone : (uint32_t)(r1 - r0));
         } while (R.next(A, lane, w, sR));
-        return;
+        if (planner)
+            return;
     }
     uint64_t x0 = (uint64_t)run * R.per;
     const uint64_t x1 = x0 + R.per;
@@ -450,6 +455,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                          : QN * (4 * (j / (QN / 4)) + g) + 4 * (j % (QN / 4));
             qx[j] = *(const f4 *)(qsrc + (qc[j] < hd ? qc[j] : 0));
         }
+        __builtin_amdgcn_sched_barrier(0);
         /* (a wave without units asks for a whole one all the same: no branch
            holds up what follows) */
         const uint32_t some = first < su + u0 ? first : su + u0 - 1;
@@ -463,6 +469,9 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         float qs2 = 1.0f, qmax = 0.0f;
 #pragma unroll
         for (int j = 0; j < NQ; j++) {
+            /* (used as loaded: the compiler else loads only where it is kept, in
+               a branch, and waits there for everything before it) */
+            asm volatile("" : "+v"(qx[j]));
             if (qrow >= rows || qc[j] >= hd)
                 qx[j] = f4{0, 0, 0, 0};
 #pragma unroll
@@ -851,9 +860,9 @@ __global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
 template <int T, int D> hipError_t launch_sel(const PagesArgs &a, hipStream_t s)
 {
     if (a.sel)
-        hipLaunchKernelGGL((pages_kernel<T, D, true>), dim3(a.n_wg + 1), dim3(kPW * 64), 0, s, a);
+        hipLaunchKernelGGL((pages_kernel<T, D, true>), dim3(a.n_wg + (a.n_seqs > 64)), dim3(kPW * 64), 0, s, a);
     else
-        hipLaunchKernelGGL((pages_kernel<T, D, false>), dim3(a.n_wg + 1), dim3(kPW * 64), 0, s, a);
+        hipLaunchKernelGGL((pages_kernel<T, D, false>), dim3(a.n_wg + (a.n_seqs > 64)), dim3(kPW * 64), 0, s, a);
     return hipGetLastError();
 }
 

@@ -156,13 +156,37 @@ template <int CTRL> __device__ __forceinline__ double dpp(double x)
         double, make_uint2(__builtin_amdgcn_update_dpp(0u, u.x, CTRL, 0xf, 0xf, false),
                            __builtin_amdgcn_update_dpp(0u, u.y, CTRL, 0xf, 0xf, false)));
 }
-/* over 16 lanes: quad_perm [1, 0, 3, 2], [2, 3, 0, 1], row_ror 8 and 4 */
-__device__ __forceinline__ double sum16(double x)
+/* one step of a sum over 16 lanes (CTRL pairs each lane with its partner) ... */
+template <int CTRL> __device__ __forceinline__ double step(double x) { return x + dpp<CTRL>(x); }
+/* ... and of two sums at once: the lanes with `hi` go on with b, the others with
+   a */
+template <int CTRL> __device__ __forceinline__ double step2(double a, double b, bool hi)
 {
-    x += dpp<0xB1>(x);
-    x += dpp<0x4E>(x);
-    x += dpp<0x128>(x);
-    return x + dpp<0x124>(x);
+    return (hi ? b : a) + dpp<CTRL>(hi ? a : b);
+}
+template <int CTRL> __device__ __forceinline__ float max_dpp(float x)
+{
+    return fmaxf(x, __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(x), CTRL, 0xf,
+                                                                0xf, false)));
+}
+/* The sums over 16 lanes of s[0 .. N), and the largest of them as floats, in
+   every lane: row_ror 8, row_half_mirror (7 - l in 8 lanes), then quad_perm [2, 3,
+   0, 1] and [1, 0, 3, 2] */
+template <uint32_t N> __device__ __forceinline__ float largest16(const double *s, uint32_t c)
+{
+    double x;
+    if constexpr (N == 4)
+        x = step2<0x141>(step2<0x128>(s[0], s[1], c & 8), step2<0x128>(s[2], s[3], c & 8), c & 4);
+    else if constexpr (N == 2)
+        x = step<0x141>(step2<0x128>(s[0], s[1], c & 8));
+    else
+        x = step<0x141>(step<0x128>(s[0]));
+    float y = (float)step<0xB1>(step<0x4E>(x));
+    if constexpr (N >= 2)
+        y = max_dpp<0x128>(y);
+    if constexpr (N == 4)
+        y = max_dpp<0x141>(y);
+    return y;
 }
 
 constexpr uint32_t kScoreBlocks = 16;  /* blocks a workgroup at once, 16 lanes each */
@@ -171,7 +195,8 @@ constexpr uint32_t kScoreBlocks = 16;  /* blocks a workgroup at once, 16 lanes e
  * A block's 16 lanes take 8 dimensions of every 128 each; HC: 128s of the head
  * size. The query of 4 / HC heads stays in registers, as doubles and as the mask
  * of its positive numbers, while the lanes go from block to block, the next
- * block's bounds asked for before this one's are used: a number and head are a
+ * block's bounds asked for before this one's are used (their pages 16 blocks at
+ * a time: a load less to wait for at each): a number and head are a
  * bit select, a conversion and a multiply-add. A group of more heads goes over
  * the blocks again.
  */
@@ -193,9 +218,15 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
 #pragma unroll
     for (int i = 0; i < HC; i++)
         in[i] = 128 * i + 8 * c < hd;
-    auto boxes = [&](uint32_t j, h8 *lo, h8 *hi) {
-        uint32_t pid = table[j];
-        pid = pid < A.n_pages ? pid : 0;
+    /* the pages of the next 16 blocks that these lanes come to, one a lane */
+    uint32_t pids = 0;
+    auto fetch = [&](uint32_t j) {
+        const uint64_t mine = j + (uint64_t)c * step;
+        pids = table[mine < bl.n ? mine : bl.n - 1];
+        pids = pids < A.n_pages ? pids : 0;
+    };
+    auto boxes = [&](uint32_t k, h8 *lo, h8 *hi) {
+        const uint32_t pid = __shfl(pids, (int)((tid & 48) + k % 16), 64);
         const _Float16 *const box = A.bounds + ((size_t)pid * A.n_kv + kvh) * 2 * hd;
 #pragma unroll
         for (int i = 0; i < HC; i++) {
@@ -204,6 +235,7 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
             hi[i] = *(const h8 *)(box + hd + d);
         }
     };
+    fetch(j0);
     for (uint32_t h0 = 0; h0 < A.group; h0 += HT) {
         const float *const q =
             A.q + (size_t)sv.row * A.q_stride + ((size_t)kvh * A.group + h0) * hd;
@@ -225,8 +257,10 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
                 }
             }
         h8 lo[HC], hi[HC];
-        boxes(j0, lo, hi);
-        for (uint32_t j = j0; j < bl.n; j += step) {
+        if (h0 && (bl.n - 1 - j0) / step >= 16)
+            fetch(j0);
+        boxes(0, lo, hi);
+        for (uint32_t j = j0, k = 1; j < bl.n; j += step, k++) {
             uint32_t l[HC][8], u[HC][8];
 #pragma unroll
             for (int i = 0; i < HC; i++)
@@ -235,9 +269,12 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
                     l[i][e] = __float_as_uint((float)lo[i][e]);
                     u[i][e] = __float_as_uint((float)hi[i][e]);
                 }
-            if (j + step < bl.n)
-                boxes(j + step, lo, hi);
-            float best = -INFINITY;
+            if (j + step < bl.n) {
+                if (k % 16 == 0)
+                    fetch(j + step);
+                boxes(k, lo, hi);
+            }
+            double sum[HT];
 #pragma unroll
             for (uint32_t h = 0; h < HT; h++) {
                 double s = 0.0;
@@ -249,10 +286,10 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
                         const float b = __uint_as_float((u[i][e] & k) | (l[i][e] & ~k));
                         s = __builtin_fma(x[h][i][e], (double)b, s);
                     }
-                const float y = (float)sum16(s);
-                if (h0 + h < A.group)
-                    best = fmaxf(best, y);
+                /* (a head past the group: the first one again) */
+                sum[h] = h0 + h < A.group ? s : sum[0];
             }
+            const float best = largest16<HT>(sum, c);
             if (c == 0)
                 out[j] = h0 == 0 ? best : fmaxf(best, out[j]);
         }
@@ -459,11 +496,12 @@ hipError_t launch_bounds(const BoundsArgs &a, hipStream_t s)
 
 hipError_t launch_select(const SelectArgs &a, hipStream_t s)
 {
-    /* as many workgroups as hold the table's blocks once, no more than fill
-       the device eight times (max_pages may be far above the lengths) */
+    /* as many workgroups as hold the table's blocks once, no more than fill the
+       device (max_pages may be far above the lengths, and each workgroup makes
+       its query first) */
     const uint32_t pairs = a.n_seqs * a.n_kv;
     uint32_t x = (a.max_pages + kScoreBlocks - 1) / kScoreBlocks;
-    const uint32_t most = pairs < 8 * a.cus ? 8 * a.cus / pairs : 1;
+    const uint32_t most = pairs < 4 * a.cus ? 4 * a.cus / pairs : 1;
     x = x < most ? x : most;
     const dim3 grid(x, a.n_kv, a.n_seqs);
     if (a.hd <= 128)
