@@ -84,11 +84,6 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t x)
     x += shifted<0x143, 0xc>(x);
     return x;
 }
-__device__ __forceinline__ uint64_t uniform(uint64_t x)
-{
-    return (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
-           __builtin_amdgcn_readfirstlane((uint32_t)x);
-}
 __device__ __forceinline__ uint32_t sum_wave(uint32_t x)
 {
     return __builtin_amdgcn_readlane(scan_wave(x), 63);
@@ -111,9 +106,10 @@ constexpr uint32_t kLeastUnits = kPW;
  */
 struct RunsLds {
     uint32_t row[64], lo[64], end[64], units[64];
-    uint64_t from[64], to[64];   /* a sequence's units in the launch's */
+    uint32_t from[64], to[64];   /* a sequence's units in the launch's */
 };
 
+/* (units count in 32 bits: janas_attn_pages_run refuses tables that hold more) */
 template <bool SEL> struct Runs {
     uint32_t i0, per, whole;     /* units a run; each sequence in whole runs */
 
@@ -125,14 +121,15 @@ template <bool SEL> struct Runs {
         s = seq_view(A, i);
         return seq_units<SEL>(A, s);
     }
+    __device__ __forceinline__ uint32_t runs_of(uint32_t u) const
+    {
+        return u ? (u - 1) / per + 1 : 0;
+    }
     /* sequences i0 .. i0 + 63, which follow on `before` units, to LDS */
-    __device__ __forceinline__ void place(const SeqView &s, uint32_t u, uint64_t before,
+    __device__ __forceinline__ void place(const SeqView &s, uint32_t u, uint32_t before,
                                           uint32_t lane, uint32_t w, RunsLds &L) const
     {
-        const uint64_t r = whole && u ? (uint64_t)((u - 1) / per + 1) * per : u;
-        /* (64 lanes of less than 2^32: in halves) */
-        const uint64_t to = before + (uint64_t)scan_wave((uint32_t)(r >> 16)) * 65536 +
-                            scan_wave((uint32_t)r & 0xFFFF);
+        const uint32_t r = whole ? runs_of(u) * per : u, to = before + scan_wave(r);
         if (w == 0) {
             L.row[lane] = s.part ? s.row : kNone;
             L.lo[lane] = s.lo;
@@ -146,20 +143,17 @@ template <bool SEL> struct Runs {
     __device__ __forceinline__ void begin(const PagesArgs &A, uint32_t lane, uint32_t w, RunsLds &L)
     {
         SeqView s;
-        uint32_t u = 0;
-        uint64_t total = 0;
+        uint32_t u = 0, total = 0, runs = 0;
         for (i0 = 0; i0 < A.n_seqs; i0 += 64) {
             u = units(A, i0 + lane, s);
-            total += (uint64_t)sum_wave(u >> 16) * 65536 + sum_wave(u & 0xFFFF);
+            total += sum_wave(u);
         }
-        uint64_t p = (total + A.share - 1) / A.share;
-        p = p < kLeastUnits ? kLeastUnits : p;
-        per = p < 0x10000000u ? (uint32_t)p : 0x10000000u;
-        uint64_t runs = 0;
+        per = (total + A.share - 1) / A.share;
+        per = per > kLeastUnits ? per : kLeastUnits;
         for (i0 = 0; i0 < A.n_seqs; i0 += 64) {
             if (A.n_seqs > 64)
                 u = units(A, i0 + lane, s);
-            runs += sum_wave(u ? (u - 1) / per + 1 : 0);
+            runs += sum_wave(runs_of(u));
         }
         whole = runs <= A.share;
         i0 = 0;
@@ -172,7 +166,7 @@ template <bool SEL> struct Runs {
     {
         if (i0 + 64 >= A.n_seqs)
             return false;
-        const uint64_t before = L.to[63];
+        const uint32_t before = L.to[63];
         __syncthreads();
         i0 += 64;
         SeqView s;
@@ -300,17 +294,16 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         const uint32_t lane = thread & 63;
         do {
             const uint32_t i = R.i0 + lane, u = sR.units[lane];
-            const uint64_t r0 = sR.from[lane] / R.per;
-            const uint64_t r1 = u ? (sR.from[lane] + u - 1) / R.per + 1 : r0;
+            const uint32_t r0 = sR.from[lane] / R.per;
+            const uint32_t r1 = u ? (sR.from[lane] + u - 1) / R.per + 1 : r0;
             if (w == kPW - 1 && i < A.n_seqs)
-                A.plan[i] = make_uint2((uint32_t)r0 + i,
-                                       sR.row[lane] == kNone ? kNone : (uint32_t)(r1 - r0));
+                A.plan[i] = make_uint2(r0 + i, sR.row[lane] == kNone ? kNone : r1 - r0);
         } while (R.next(A, lane, w, sR));
         if (planner)
             return;
     }
-    uint64_t x0 = (uint64_t)run * R.per;
-    const uint64_t x1 = x0 + R.per;
+    uint32_t x0 = run * R.per;
+    const uint32_t x1 = x0 + R.per;
     /* sequence after sequence of the run */
     for (;;) {
         /* (the thread's number unknown to the compiler: what follows from it is made
@@ -325,7 +318,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         const uint32_t hl = (uint32_t)__builtin_ctzll(hit);
         const uint32_t si = R.i0 + hl;
         const uint32_t su = __builtin_amdgcn_readfirstlane(sR.units[hl]);
-        const uint64_t s0 = uniform(sR.from[hl]), s1 = uniform(sR.to[hl]);
+        const uint32_t s0 = __builtin_amdgcn_readfirstlane(sR.from[hl]);
+        const uint32_t s1 = __builtin_amdgcn_readfirstlane(sR.to[hl]);
         if (s0 >= x1)
             return;
         SeqView sv;
@@ -333,8 +327,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         sv.lo = __builtin_amdgcn_readfirstlane(sR.lo[hl]);
         sv.end = __builtin_amdgcn_readfirstlane(sR.end[hl]);
         /* its units [ua, ub) are this run's; `only`: all of them */
-        const uint32_t ua = x0 > s0 ? (uint32_t)(x0 - s0) : 0;
-        const uint32_t ub = x1 - s0 < su ? (uint32_t)(x1 - s0) : su;
+        const uint32_t ua = x0 > s0 ? x0 - s0 : 0;
+        const uint32_t ub = x1 - s0 < su ? x1 - s0 : su;
         const bool only = ua == 0 && ub == su;
         const uint32_t hd = A.hd, G = A.group, rowb = hd * EB;
         const uint32_t kvh = tile / A.rtiles, r0 = tile % A.rtiles * ROWS;
@@ -416,21 +410,26 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             if constexpr (SCALED)
                 ks = *(const f4 *)(A.ks + x.row + 4 * g);
         };
-        /* value rows past the sequence's are read as its last one (they weigh 0,
-           but what is there may be no number) */
+        /* value rows that are not in sight are read as the first or last one that is
+           (they weigh 0, but what is there may be no number) */
         auto load_v = [&](const Unit &x) {
-            const uint32_t hi = x.pos < sv.end ? (sv.end - 1 - x.pos < 15 ? sv.end - 1 - x.pos : 15) : 0;
-            const uint32_t lo = x.pos < sv.lo ? (sv.lo - x.pos < 15 ? sv.lo - x.pos : 15) : 0;
             const char *const p = (const char *)A.v + x.row * rowb;
+            uint32_t r[4] = {4 * g * rowb, (4 * g + 1) * rowb, (4 * g + 2) * rowb, (4 * g + 3) * rowb};
+            if (x.pos < sv.lo || x.pos + kUnit > sv.end) {
+                const uint32_t past = sv.end - 1 - x.pos, short_ = sv.lo - x.pos;
+                const uint32_t hi = x.pos < sv.end ? (past < 15 ? past : 15) : 0;
+                const uint32_t lo = x.pos < sv.lo ? (short_ < 15 ? short_ : 15) : 0;
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                uint32_t r = 4 * g + j;
-                r = r > lo ? r : lo;
-                r = r < hi ? r : hi;
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t y = 4 * g + j > lo ? 4 * g + j : lo;
+                    r[j] = (y < hi ? y : hi) * rowb;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int u = 0; u < VU; u++)
-                    vr[j][u] = __builtin_nontemporal_load((const VT *)(p + r * rowb + vat[u]));
-            }
+                    vr[j][u] = __builtin_nontemporal_load((const VT *)(p + (r[j] + vat[u])));
             if constexpr (SCALED)
                 vs = *(const f4 *)(A.vs + x.row + 4 * g);
         };
@@ -445,15 +444,16 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         /* LDS: the workgroup's rows once, 256 / ROWS lanes a row, words of four */
         constexpr int TPR = kPW * 64 / ROWS, NQ = QLDS ? D / (4 * TPR) : KL * QN / 4;
         const uint32_t qrow = QLDS ? tid / TPR : F32 ? n : n >> 1;
-        const float *const qsrc =
-            A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0 + (qrow < rows ? qrow : 0)) * hd;
+        const char *const qsrc =
+            (const char *)(A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0) * hd);
+        const uint32_t qat = (qrow < rows ? qrow : 0) * hd;
         f4 qx[NQ];
         uint32_t qc[NQ];
 #pragma unroll
         for (int j = 0; j < NQ; j++) {
             qc[j] = QLDS ? 4 * (tid % TPR + TPR * j)
                          : QN * (4 * (j / (QN / 4)) + g) + 4 * (j % (QN / 4));
-            qx[j] = *(const f4 *)(qsrc + (qc[j] < hd ? qc[j] : 0));
+            qx[j] = *(const f4 *)(qsrc + 4 * (qat + (qc[j] < hd ? qc[j] : 0)));
         }
         __builtin_amdgcn_sched_barrier(0);
         /* (a wave without units asks for a whole one all the same: no branch

@@ -295,6 +295,9 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
         (c->out_q8k && (uint64_t)g.n_head * g.hd % JANAS_ATTN_QK))
         return JANAS_ATTN_EINVAL;
     const Parts t = parts_of(g, p);
+    /* a call's units of 16 positions (and what rounds them up) in 32 bits */
+    if ((uint64_t)p->n_seqs * p->max_pages * (p->page / 16) >= 1ull << 31)
+        return JANAS_ATTN_ERANGE;
     const uint64_t cols = pages_merge_cols(p->n_seqs, g.n_head, g.hd);
     const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + cols - 1) / cols);
     const uint64_t rows = c->row ? c->n_rows : p->n_seqs;

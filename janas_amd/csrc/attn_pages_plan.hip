@@ -5,8 +5,8 @@
  *
  * Two sums over the sequences decide everything: the tokens before a sequence
  * (its first packed row) and the pages asked for before it (where in the stack
- * of free pages its own begin). One workgroup takes them, 1024 sequences at a
- * time, and for a small step (a decode's) writes tables and slots too: one
+ * of free pages its own begin). One workgroup takes them, 64 or 1024 sequences
+ * at a time, and for a small step (a decode's) writes tables and slots too: one
  * launch. A large step's tokens and pages go to a second kernel, a thread each,
  * which finds a token's sequence in the first rows by halving.
  *
@@ -21,18 +21,34 @@
 namespace janas {
 namespace {
 
-constexpr uint32_t kPlanThreads = 1024;
-constexpr uint32_t kPlanWaves = kPlanThreads / 64;
+/* the sum over the lanes up to and with this one (row_shr 1, 2, 4, 8, then
+   row_bcast 15 and 31) */
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t shifted(uint32_t x)
+{
+    return __builtin_amdgcn_update_dpp(0u, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x)
+{
+    x += shifted<0x111, 0xf>(x);
+    x += shifted<0x112, 0xf>(x);
+    x += shifted<0x114, 0xf>(x);
+    x += shifted<0x118, 0xf>(x);
+    x += shifted<0x142, 0xa>(x);
+    x += shifted<0x143, 0xc>(x);
+    return x;
+}
 
-/* the sum of x over the threads before this one; total: over all */
-__device__ uint64_t scan_group(uint64_t x, uint64_t *lds, uint64_t &total)
+/* the sum of x (below 2^32) over the threads before this one; total: over all */
+template <uint32_t WAVES>
+__device__ __forceinline__ uint64_t scan_group(uint32_t x, uint64_t *lds, uint64_t &total)
 {
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    uint64_t s = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long)s, o, 64);
-        s += lane >= (uint32_t)o ? y : 0;
+    /* (64 lanes: in halves) */
+    const uint64_t s = (uint64_t)scan_wave(x >> 16) * 65536 + scan_wave(x & 0xFFFF);
+    if constexpr (WAVES == 1) {
+        total = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(s >> 32), 63) << 32 |
+                __builtin_amdgcn_readlane((uint32_t)s, 63);
+        return s - x;
     }
     if (lane == 63)
         lds[w] = s;
@@ -40,7 +56,7 @@ __device__ uint64_t scan_group(uint64_t x, uint64_t *lds, uint64_t &total)
     uint64_t before = 0;
     total = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kPlanWaves; i++) {
+    for (uint32_t i = 0; i < WAVES; i++) {
         const uint64_t y = lds[i];
         before += i < w ? y : 0;
         total += y;
@@ -61,35 +77,45 @@ __device__ __forceinline__ uint32_t stack_page(const PlanArgs &A, uint64_t top, 
     return k < top ? A.free_pages[top - 1 - k] : 0;
 }
 
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs A)
+/*
+ * WAVES x 64 sequences at a time: one wave where there are no more (no barriers
+ * between its steps but the hardware's own), else 16. A step's three reads -
+ * counts, then lengths' pages - are all that its chain waits for.
+ */
+template <uint32_t WAVES>
+__global__ __launch_bounds__(WAVES * 64) void plan_kernel(const PlanArgs A)
 {
-    __shared__ uint64_t sScan[kPlanWaves];
-    __shared__ uint32_t sOld[kPlanThreads], sNew[kPlanThreads], sNeed[kPlanThreads];
-    __shared__ uint32_t sTok[kPlanThreads];
-    __shared__ uint64_t sTake[kPlanThreads];
+    constexpr uint32_t THREADS = WAVES * 64;
+    __shared__ uint64_t sScan[WAVES];
+    __shared__ uint32_t sOld[THREADS], sNew[THREADS], sNeed[THREADS], sTok[THREADS], sOk[THREADS];
+    __shared__ uint64_t sTake[THREADS];
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const uint64_t room = (uint64_t)A.max_pages << A.page_log;
     uint64_t top = *A.n_free;
+    /* the first THREADS sequences' */
+    const uint32_t new0 = tid < A.n_seqs ? A.n_new[tid] : 0;
+    const uint32_t len0 = tid < A.n_seqs ? A.len[tid] : 0;
     top = top < A.n_pages ? top : A.n_pages;
     /* every thread has the count before one of them may change it */
     __syncthreads();
 
     /* ---- released pages onto the stack, sequence after sequence ---- */
-    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += kPlanThreads) {
+    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += THREADS) {
         const uint32_t i = i0 + tid;
-        const bool gone = i < A.n_seqs && A.n_new[i] == kRelease;
+        const bool gone = i < A.n_seqs && (i0 ? A.n_new[i] : new0) == kRelease;
         if (!__syncthreads_or(gone))
             continue;
-        uint64_t gave = 0, all;
+        uint64_t all;
+        uint32_t gave = 0;
         if (gone) {
-            gave = blocks_of(A.len[i], A.page_log);
-            gave = gave < A.max_pages ? gave : A.max_pages;
+            const uint64_t b = blocks_of(A.len[i], A.page_log);
+            gave = b < A.max_pages ? (uint32_t)b : A.max_pages;
         }
-        const uint64_t at = top + scan_group(gave, sScan, all);
-        sNeed[tid] = (uint32_t)gave;
+        const uint64_t at = top + scan_group<WAVES>(gave, sScan, all);
+        sNeed[tid] = gave;
         sTake[tid] = at;
         __syncthreads();
-        for (uint32_t k = w; k < kPlanThreads && i0 + k < A.n_seqs; k += kPlanWaves) {
+        for (uint32_t k = w; k < THREADS && i0 + k < A.n_seqs; k += WAVES) {
             const uint32_t n = sNeed[k];
             const uint32_t *const row = A.table + (size_t)(i0 + k) * A.max_pages;
             for (uint32_t b = lane; b < n; b += 64)
@@ -98,90 +124,83 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs A)
         }
         top += all;
         top = top < A.n_pages ? top : A.n_pages;
+        /* what was pushed is read below, by other threads */
+        __threadfence_block();
         __syncthreads();
     }
-    /* what was pushed is read below, by other threads */
-    __threadfence_block();
-    __syncthreads();
 
     /* ---- tokens and pages ---- */
     uint64_t tok = 0, asked = 0, took = 0;
-    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += kPlanThreads) {
+    for (uint32_t i0 = 0; i0 < A.n_seqs; i0 += THREADS) {
         const uint32_t i = i0 + tid;
-        uint64_t old = 0, add = 0, all_tok, all_need;
-        if (i < A.n_seqs) {
-            old = A.len[i];
-            add = A.n_new[i];
+        const bool mine = i < A.n_seqs;
+        uint32_t old = 0, add = 0;
+        uint64_t all_tok, all_need;
+        if (mine) {
+            old = i0 ? A.len[i] : len0;
+            add = i0 ? A.n_new[i] : new0;
             if (add == kRelease)
                 old = add = 0;
         }
-        const uint64_t first = tok + scan_group(add, sScan, all_tok);
-        const bool fits = old + add <= room && first + add <= A.max_tokens;
-        const uint64_t have = blocks_of(old, A.page_log);
-        const uint64_t need = fits ? blocks_of(old + add, A.page_log) - have : 0;
-        const uint64_t before = asked + scan_group(need, sScan, all_need);
+        const uint64_t first = tok + scan_group<WAVES>(add, sScan, all_tok);
+        const bool fits = (uint64_t)old + add <= room && first + add <= A.max_tokens;
+        const uint32_t have = (uint32_t)blocks_of(old, A.page_log);
+        const uint32_t need = fits ? (uint32_t)blocks_of((uint64_t)old + add, A.page_log) - have : 0;
+        const uint64_t before = asked + scan_group<WAVES>(need, sScan, all_need);
         const bool ok = fits && (need == 0 || before + need <= top);
         /* the pages taken up to here: once a sequence found too few, none */
         uint64_t take = before;
         uint64_t all_take = all_need;
-        if (asked + all_need > top) {
-            take = took + scan_group(ok ? need : 0, sScan, all_take);
+        if (asked + all_need > top)
+            take = took + scan_group<WAVES>(ok ? need : 0, sScan, all_take);
+        const bool many = mine && (add > 1 || need > 1);
+        if (A.whole && mine && !many) {
+            /* a token or none, a page or none */
+            uint32_t *const row = A.table + (size_t)i * A.max_pages;
+            uint32_t page = 0;
+            if (ok && add)
+                page = need ? stack_page(A, top, take) : row[old >> A.page_log];
+            if (ok && need)
+                row[have] = page;
+            if (add && first < A.max_tokens) {
+                const uint32_t in = old & ((1u << A.page_log) - 1);
+                A.slot[first] = ok ? (page << A.page_log) + in : kNone;
+                A.pos[first] = ok ? old : 0;
+                A.seq[first] = i;
+            }
         }
-        if (i < A.n_seqs) {
+        if (mine) {
             A.start[i] = first < 0xFFFFFFFFu ? (uint32_t)first : 0xFFFFFFFFu;
             A.taken[i] = (uint32_t)take;
-            A.granted[i] = ok ? (uint32_t)add : 0;
-            A.len_out[i] = (uint32_t)(old + (ok ? add : 0));
+            A.granted[i] = ok ? add : 0;
+            A.len_out[i] = old + (ok ? add : 0);
         }
-        if (A.whole) {
-            const bool mine = i < A.n_seqs;
-            sOld[tid] = (uint32_t)old;
-            sNeed[tid] = ok ? (uint32_t)need : 0;
-            sTake[tid] = take;
+        if (A.whole && __syncthreads_or(many)) {
+            /* the others, a wave a sequence */
+            sOld[tid] = old;
+            sNew[tid] = many ? (add < A.max_tokens ? add : A.max_tokens) : 0;
+            sNeed[tid] = many && ok ? need : 0;
             sTok[tid] = first < A.max_tokens ? (uint32_t)first : A.max_tokens;
-            sNew[tid] = mine ? (add < A.max_tokens ? (uint32_t)add : A.max_tokens) : 0;
-            const bool many = mine && (add > 1 || need > 1);
-            if (mine && !many) {
-                /* a token or none, a page or none */
-                uint32_t *const row = A.table + (size_t)i * A.max_pages;
-                if (ok && need)
-                    row[have] = stack_page(A, top, take);
-                if (add && first < A.max_tokens) {
-                    uint32_t s = kNone;
-                    if (ok) {
-                        const uint32_t b = (uint32_t)old >> A.page_log;
-                        const uint32_t p = need ? stack_page(A, top, take) : row[b];
-                        s = (p << A.page_log) + ((uint32_t)old & ((1u << A.page_log) - 1));
+            sTake[tid] = take;
+            sOk[tid] = ok;
+            __syncthreads();
+            for (uint32_t k = w; k < THREADS && i0 + k < A.n_seqs; k += WAVES) {
+                const uint32_t n = sNew[k], q = sNeed[k], at = sTok[k], o = sOld[k];
+                const uint32_t h = (uint32_t)blocks_of(o, A.page_log);
+                uint32_t *const row = A.table + (size_t)(i0 + k) * A.max_pages;
+                for (uint32_t b = lane; b < q; b += 64)
+                    row[h + b] = stack_page(A, top, sTake[k] + b);
+                for (uint32_t t = lane; t < n && at + t < A.max_tokens; t += 64) {
+                    uint32_t s = kNone, p = 0;
+                    if (sOk[k]) {
+                        p = o + t;
+                        const uint32_t b = p >> A.page_log;
+                        s = b < h ? row[b] : stack_page(A, top, sTake[k] + b - h);
+                        s = (s << A.page_log) + (p & ((1u << A.page_log) - 1));
                     }
-                    A.slot[first] = s;
-                    A.pos[first] = ok ? (uint32_t)old : 0;
-                    A.seq[first] = i;
-                }
-            }
-            if (__syncthreads_or(many)) {
-                /* the others, a wave a sequence */
-                for (uint32_t k = w; k < kPlanThreads && i0 + k < A.n_seqs; k += kPlanWaves) {
-                    const uint32_t n = sNew[k], q = sNeed[k];
-                    if (n <= 1 && q <= 1)
-                        continue;
-                    const uint32_t at = sTok[k], o = sOld[k];
-                    const uint32_t h = (uint32_t)blocks_of(o, A.page_log);
-                    const bool given = (uint64_t)o + n <= room && A.granted[i0 + k] != 0;
-                    uint32_t *const row = A.table + (size_t)(i0 + k) * A.max_pages;
-                    for (uint32_t b = lane; b < q; b += 64)
-                        row[h + b] = stack_page(A, top, sTake[k] + b);
-                    for (uint32_t t = lane; t < n && at + t < A.max_tokens; t += 64) {
-                        uint32_t s = kNone, p = 0;
-                        if (given) {
-                            p = o + t;
-                            const uint32_t b = p >> A.page_log;
-                            s = b < h ? row[b] : stack_page(A, top, sTake[k] + b - h);
-                            s = (s << A.page_log) + (p & ((1u << A.page_log) - 1));
-                        }
-                        A.slot[at + t] = s;
-                        A.pos[at + t] = p;
-                        A.seq[at + t] = i0 + k;
-                    }
+                    A.slot[at + t] = s;
+                    A.pos[at + t] = p;
+                    A.seq[at + t] = i0 + k;
                 }
             }
             __syncthreads();
@@ -196,7 +215,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_kernel(const PlanArgs A)
         *A.n_free_out = (uint32_t)(top - took);
     }
     if (A.whole)
-        for (uint64_t t = tok + tid; t < A.max_tokens; t += kPlanThreads) {
+        for (uint64_t t = tok + tid; t < A.max_tokens; t += THREADS) {
             A.slot[t] = kNone;
             A.pos[t] = A.seq[t] = 0;
         }
@@ -259,8 +278,13 @@ __global__ __launch_bounds__(256) void plan_fill_kernel(const PlanArgs A, uint32
 
 hipError_t launch_plan(PlanArgs a, hipStream_t s)
 {
-    a.whole = a.max_tokens <= 4096;
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a);
+    /* what the first kernel's waves write in about the time of a launch: a row or
+       so a lane */
+    a.whole = a.max_tokens <= (a.n_seqs <= 64 ? 256 : 4096);
+    if (a.n_seqs <= 64)
+        hipLaunchKernelGGL(plan_kernel<1>, dim3(1), dim3(64), 0, s, a);
+    else
+        hipLaunchKernelGGL(plan_kernel<16>, dim3(1), dim3(1024), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.whole)
         return e;

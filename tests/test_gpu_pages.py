@@ -70,7 +70,9 @@ PLANS = [(1, 0, 1, 16, 1, 1, 0, 1.0), (1, 16, 1, 16, 1, 1, 0, 1.0), (48, 500, 1,
          (33, 90, 40, 16, 3, 30, 0, 1.0), (33, 90, 40, 32, 0, 300, 2, 0.6),
          (9, 4000, 2000, 16, 200, 2000, 2, 1.1), (61, 700, 900, 128, 9, 100, 5, 1.0),
          (61, 700, 900, 256, 1, 1000, 60, 0.8), (1300, 100, 1, 16, 1, 1500, 50, 1.0),
-         (2100, 60, 9, 32, 1, 900, 100, 1.0), (3, 20, 0, 16, 1, 2, 0, 1.0)]
+         (2100, 60, 9, 32, 1, 900, 100, 1.0), (3, 20, 0, 16, 1, 2, 0, 1.0),
+         (64, 40, 5, 16, 1, 90, 7, 1.0), (65, 40, 5, 16, 1, 90, 7, 1.0),
+         (12, 90, 200, 16, 8, 60, 3, 1.0)]
 
 
 @pytest.mark.parametrize("case", range(len(PLANS)))
