@@ -77,10 +77,25 @@ __device__ __forceinline__ uint32_t stack_page(const PlanArgs &A, uint64_t top, 
     return k < top ? A.free_pages[top - 1 - k] : 0;
 }
 
+/* the last i of n with at[i] <= x (at[0] = 0) */
+__device__ __forceinline__ uint32_t last_at(const uint32_t *at, uint32_t n, uint32_t x)
+{
+    uint32_t lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (at[mid] <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
 /*
- * WAVES x 64 sequences at a time: one wave where there are no more (no barriers
- * between its steps but the hardware's own), else 16. A step's three reads -
- * counts, then lengths' pages - are all that its chain waits for.
+ * WAVES x 64 sequences at a time. A step of a token or none for each of up to 64
+ * takes one wave, whose scans need no LDS: what is left of its time is a launch
+ * and two round trips, the counts and the pages (8.4 -> 3.0 us for 48 sequences,
+ * against 16 waves).
  */
 template <uint32_t WAVES>
 __global__ __launch_bounds__(WAVES * 64) void plan_kernel(const PlanArgs A)
@@ -111,16 +126,26 @@ __global__ __launch_bounds__(WAVES * 64) void plan_kernel(const PlanArgs A)
             const uint64_t b = blocks_of(A.len[i], A.page_log);
             gave = b < A.max_pages ? (uint32_t)b : A.max_pages;
         }
-        const uint64_t at = top + scan_group<WAVES>(gave, sScan, all);
-        sNeed[tid] = gave;
-        sTake[tid] = at;
+        /* where each one's begin among them; then a thread a page (4 at a time: the
+           reads before the writes), its sequence found by halving */
+        const uint64_t at = scan_group<WAVES>(gave, sScan, all);
+        sTok[tid] = at < 0xFFFFFFFFu ? (uint32_t)at : 0xFFFFFFFFu;
         __syncthreads();
-        for (uint32_t k = w; k < THREADS && i0 + k < A.n_seqs; k += WAVES) {
-            const uint32_t n = sNeed[k];
-            const uint32_t *const row = A.table + (size_t)(i0 + k) * A.max_pages;
-            for (uint32_t b = lane; b < n; b += 64)
-                if (sTake[k] + b < A.n_pages)
-                    A.free_pages[sTake[k] + b] = row[b];
+        const uint32_t n = A.n_seqs - i0 < THREADS ? A.n_seqs - i0 : THREADS;
+        /* (what the stack has room for: all, unless a page is in two places) */
+        const uint32_t fit = (uint32_t)(all < A.n_pages - top ? all : A.n_pages - top);
+        for (uint32_t f0 = tid; f0 < fit; f0 += 4 * THREADS) {
+            uint32_t page[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t f = f0 + e * THREADS < fit ? f0 + e * THREADS : fit - 1;
+                const uint32_t k = last_at(sTok, n, f);
+                page[e] = A.table[(size_t)(i0 + k) * A.max_pages + (f - sTok[k])];
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++)
+                if (f0 + e * THREADS < fit)
+                    A.free_pages[top + f0 + e * THREADS] = page[e];
         }
         top += all;
         top = top < A.n_pages ? top : A.n_pages;
@@ -221,51 +246,48 @@ __global__ __launch_bounds__(WAVES * 64) void plan_kernel(const PlanArgs A)
         }
 }
 
-/* the last i of n with at[i] <= x (at[0] = 0) */
-__device__ __forceinline__ uint32_t last_at(const uint32_t *at, uint32_t n, uint32_t x)
-{
-    uint32_t lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (at[mid] <= x)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return lo;
-}
-
 /* The tables' and the tokens' part of a large step: workgroups of 256 threads,
    the first n_tok of them over tokens, the rest over taken pages. It reads
    what plan_kernel left; a new block's page comes from the stack, not from the
    table, which other workgroups write. */
+constexpr uint32_t kFillSeqs = 1024;   /* sequences whose sums fit LDS */
+
 __global__ __launch_bounds__(256) void plan_fill_kernel(const PlanArgs A, uint32_t n_tok)
 {
-    const uint32_t took = A.taken[A.n_seqs];
+    __shared__ uint32_t sAt[kFillSeqs];
+    const bool pages = blockIdx.x >= n_tok;
+    const uint32_t *at = pages ? A.taken : A.start;
+    const uint32_t took = A.taken[A.n_seqs], tokens = A.start[A.n_seqs];
     const uint64_t top = (uint64_t)*A.n_free_out + took;
-    if (blockIdx.x >= n_tok) {
+    if (A.n_seqs <= kFillSeqs) {
+        for (uint32_t i = threadIdx.x; i < A.n_seqs; i += 256)
+            sAt[i] = at[i];
+        __syncthreads();
+        at = sAt;
+    }
+    if (pages) {
         const uint32_t k = (blockIdx.x - n_tok) * 256 + threadIdx.x;
         if (k >= took)
             return;
-        const uint32_t i = last_at(A.taken, A.n_seqs, k);
+        const uint32_t i = last_at(at, A.n_seqs, k);
         const uint32_t h = (uint32_t)blocks_of(A.len_out[i] - A.granted[i], A.page_log);
-        A.table[(size_t)i * A.max_pages + h + (k - A.taken[i])] = stack_page(A, top, k);
+        A.table[(size_t)i * A.max_pages + h + (k - at[i])] = stack_page(A, top, k);
         return;
     }
     const uint32_t t = blockIdx.x * 256 + threadIdx.x;
     if (t >= A.max_tokens)
         return;
     uint32_t s = kNone, p = 0, i = 0;
-    if (t < A.start[A.n_seqs]) {
-        i = last_at(A.start, A.n_seqs, t);
-        const uint32_t n = A.granted[i];
+    if (t < tokens) {
+        i = last_at(at, A.n_seqs, t);
+        const uint32_t n = A.granted[i], end = A.len_out[i], take = A.taken[i];
         if (n) {
-            const uint32_t old = A.len_out[i] - n;
+            const uint32_t old = end - n;
             const uint32_t h = (uint32_t)blocks_of(old, A.page_log);
-            p = old + (t - A.start[i]);
+            p = old + (t - at[i]);
             const uint32_t b = p >> A.page_log;
             s = b < h ? A.table[(size_t)i * A.max_pages + b]
-                      : stack_page(A, top, (uint64_t)A.taken[i] + b - h);
+                      : stack_page(A, top, (uint64_t)take + b - h);
             s = (s << A.page_log) + (p & ((1u << A.page_log) - 1));
         }
     }
@@ -281,8 +303,10 @@ hipError_t launch_plan(PlanArgs a, hipStream_t s)
     /* what the first kernel's waves write in about the time of a launch: a row or
        so a lane */
     a.whole = a.max_tokens <= (a.n_seqs <= 64 ? 256 : 4096);
-    if (a.n_seqs <= 64)
+    if (a.n_seqs <= 64 && a.whole)
         hipLaunchKernelGGL(plan_kernel<1>, dim3(1), dim3(64), 0, s, a);
+    else if (a.n_seqs <= 256)
+        hipLaunchKernelGGL(plan_kernel<4>, dim3(1), dim3(256), 0, s, a);
     else
         hipLaunchKernelGGL(plan_kernel<16>, dim3(1), dim3(1024), 0, s, a);
     hipError_t e = hipGetLastError();
