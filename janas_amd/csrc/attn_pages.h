@@ -74,7 +74,7 @@ struct PagesArgs {
     uint32_t n_head, n_kv, group, hd, window, q_stride;
     uint32_t rtiles;       /* workgroups along a KV head's query rows */
     uint32_t share;        /* runs of a tile that the device holds at once */
-    uint32_t n_wg;         /* pages_runs x tiles */
+    uint32_t runs;         /* pages_runs: workgroups of a tile */
     float scale;
     int gate_mode;
 };

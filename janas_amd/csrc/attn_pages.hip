@@ -33,6 +33,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include <hip/hip_runtime.h>
 
@@ -112,6 +113,7 @@ struct RunsLds {
 /* (units count in 32 bits: janas_attn_pages_run refuses tables that hold more) */
 template <bool SEL> struct Runs {
     uint32_t i0, per, whole;     /* units a run; each sequence in whole runs */
+    uint32_t runs;               /* of the launch */
 
     static __device__ __forceinline__ uint32_t units(const PagesArgs &A, uint32_t i, SeqView &s)
     {
@@ -143,7 +145,8 @@ template <bool SEL> struct Runs {
     __device__ __forceinline__ void begin(const PagesArgs &A, uint32_t lane, uint32_t w, RunsLds &L)
     {
         SeqView s;
-        uint32_t u = 0, total = 0, runs = 0;
+        uint32_t u = 0, total = 0;
+        runs = 0;
         for (i0 = 0; i0 < A.n_seqs; i0 += 64) {
             u = units(A, i0 + lane, s);
             total += sum_wave(u);
@@ -156,6 +159,7 @@ template <bool SEL> struct Runs {
             runs += sum_wave(runs_of(u));
         }
         whole = runs <= A.share;
+        runs = whole ? runs : (total + per - 1) / per;
         i0 = 0;
         if (A.n_seqs > 64)
             u = units(A, lane, s);
@@ -210,13 +214,17 @@ template <int T, int D> struct PS {
     static constexpr int VW = VN * EB / 4;           /* words of one */
     static constexpr int NT = D / 16;                /* column tiles */
     static constexpr int DP = Elem<T>::planes;
-    /* the query's operands from head size 256 on are read from LDS at each use:
-       in registers they would cost a wave a SIMD (256) or spill (512) */
-    static constexpr bool QLDS = D >= 256;
+    /* the query's operands stay in registers; from head size 256 on they are read
+       from LDS at each use: they would cost a wave a SIMD (256) or spill (512) */
+    static constexpr bool QREG = D < 256;
     static constexpr int QROW = F32 ? D + 4 : D / 2 + 4; /* words of an LDS row */
-    static constexpr int QCOLS = 16;
     static constexpr int WAVES = pages_waves(T, D);  /* a SIMD, by registers */
 };
+
+template <bool KEEP, class V> __device__ __forceinline__ V load_once(const V *p)
+{
+    return KEEP ? *p : __builtin_nontemporal_load(p);
+}
 
 /* numbers e of four rows' V words as B operands, one a plane */
 template <int T, int VW>
@@ -264,7 +272,12 @@ __device__ __forceinline__ uint32_t exponent(float x) { return (__float_as_uint(
 
 /* ---- the kernel ---------------------------------------------------------------- */
 
-template <int T, int D, bool SEL>
+/* MULTI: a KV head's query rows take several workgroups, which read the same
+   keys and values: they are dealt to one XCD, side by side, and keep them in its
+   L2. Else every row is read once, past the caches (60 sequences at 4170
+   positions 187 -> 168 us; 32 query heads on one KV head, with the caches,
+   53.7 -> 45.4). */
+template <int T, int D, bool SEL, bool MULTI>
 __global__ __launch_bounds__(kPW * 64)
 __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const PagesArgs A)
 {
@@ -273,10 +286,20 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
     constexpr int DP = S::DP, ROWS = S::ROWS;
     constexpr bool F32 = S::F32, SCALED = S::SCALED;
     typedef typename Words<VW>::T VT;
-    __shared__ __attribute__((aligned(16))) float sO[kPW][ROWS][D];
+    /* the query's operands, and the waves' sums: from head size 256 on in the same
+       place */
+    constexpr bool QREG = S::QREG;
+    struct Apart {
+        float o[kPW][ROWS][D], q[16][S::QROW];
+    };
+    union Shared {
+        float o[kPW][ROWS][D], q[16][S::QROW];
+    };
+    __shared__ __attribute__((aligned(16))) typename std::conditional<QREG, Apart, Shared>::type sX;
+    auto &sO = sX.o;
+    auto &sQ = sX.q;
     __shared__ float sM[kPW][ROWS], sL[kPW][ROWS];
     __shared__ float sE[kPW];
-    __shared__ __attribute__((aligned(16))) float sQ[S::QLDS ? S::QCOLS : 1][S::QLDS ? S::QROW : 4];
     __shared__ float sQs[ROWS];
     __shared__ RunsLds sR;
 
@@ -284,11 +307,10 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
     /* with more than 64 sequences, one workgroup more, the first, writes the plan;
        else the first does it besides */
     const bool planner = A.n_seqs > 64;
-    const uint32_t id = blockIdx.x - (planner ? 1 : 0);
-    const uint32_t tiles = A.n_kv * A.rtiles, tile = id % tiles, run = id / tiles;
+    uint32_t run = blockIdx.z - (planner ? 1 : 0), kvh = blockIdx.y, rt = blockIdx.x;
     Runs<SEL> R;
     R.begin(A, thread & 63, w, sR);
-    if (blockIdx.x == 0) {
+    if (blockIdx.x + blockIdx.y + blockIdx.z == 0) {
         /* for the merge, each sequence's partials: the one of run x and sequence
            i has number x + i */
         const uint32_t lane = thread & 63;
@@ -299,9 +321,20 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             if (w == kPW - 1 && i < A.n_seqs)
                 A.plan[i] = make_uint2(r0 + i, sR.row[lane] == kNone ? kNone : r1 - r0);
         } while (R.next(A, lane, w, sR));
-        if (planner)
-            return;
     }
+    if (planner && blockIdx.z == 0)
+        return;
+    const uint32_t tiles = A.n_kv * A.rtiles;
+    if constexpr (MULTI) {
+        const uint32_t all = R.runs * tiles, id = (run * A.n_kv + kvh) * A.rtiles + rt;
+        if (id >= all)
+            return;
+        const uint32_t to = xcd_remap(id, all);
+        rt = to % A.rtiles;
+        kvh = to / A.rtiles % A.n_kv;
+        run = to / tiles;
+    }
+    const uint32_t tile = kvh * A.rtiles + rt;
     uint32_t x0 = run * R.per;
     const uint32_t x1 = x0 + R.per;
     /* sequence after sequence of the run */
@@ -331,7 +364,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         const uint32_t ub = x1 - s0 < su ? x1 - s0 : su;
         const bool only = ua == 0 && ub == su;
         const uint32_t hd = A.hd, G = A.group, rowb = hd * EB;
-        const uint32_t kvh = tile / A.rtiles, r0 = tile % A.rtiles * ROWS;
+        const uint32_t r0 = rt * ROWS;
         const uint32_t rows = G - r0 < ROWS ? G - r0 : ROWS;
         const uint32_t page = 1u << A.page_log, upp = page / kUnit, upp_log = A.page_log - 4;
 
@@ -406,7 +439,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             const char *const p = (const char *)A.k + x.row * rowb;
 #pragma unroll
             for (int i = 0; i < KL; i++)
-                kr[i] = __builtin_nontemporal_load((const u4 *)(p + kat[i]));
+                kr[i] = load_once<MULTI>((const u4 *)(p + kat[i]));
             if constexpr (SCALED)
                 ks = *(const f4 *)(A.ks + x.row + 4 * g);
         };
@@ -429,21 +462,19 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int u = 0; u < VU; u++)
-                    vr[j][u] = __builtin_nontemporal_load((const VT *)(p + (r[j] + vat[u])));
+                    vr[j][u] = load_once<MULTI>((const VT *)(p + (r[j] + vat[u])));
             if constexpr (SCALED)
                 vs = *(const f4 *)(A.vs + x.row + 4 * g);
         };
 
         /* ---- the query: MFMA column n's (row n / 2, plane n & 1; f32: row n) as the
-           B operand of each K load, in registers or LDS. Planes: scaled by 2^ex
-           so that the row's largest lies in [2^13, 2^14). Asked for first, made
-           when the first unit has been asked for: one round trip for the query
-           and the table, one for the unit ---- */
-        constexpr int QN = 16 / EB;      /* numbers of a K load: 16, 8 or 4 */
-        constexpr bool QLDS = S::QLDS;
-        /* LDS: the workgroup's rows once, 256 / ROWS lanes a row, words of four */
-        constexpr int TPR = kPW * 64 / ROWS, NQ = QLDS ? D / (4 * TPR) : KL * QN / 4;
-        const uint32_t qrow = QLDS ? tid / TPR : F32 ? n : n >> 1;
+           B operand of each K load. Planes: scaled by 2^ex so that the row's
+           largest lies in [2^13, 2^14). The workgroup makes them once, 256 / ROWS
+           lanes a row, words of four, through LDS; asked for first, made when the
+           first unit has been asked for: one round trip for the query and the
+           table, one for the unit ---- */
+        constexpr int TPR = kPW * 64 / ROWS, NQ = (D + 4 * TPR - 1) / (4 * TPR);
+        const uint32_t qrow = tid / TPR;
         const char *const qsrc =
             (const char *)(A.q + (size_t)sv.row * A.q_stride + (size_t)(kvh * G + r0) * hd);
         const uint32_t qat = (qrow < rows ? qrow : 0) * hd;
@@ -451,8 +482,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         uint32_t qc[NQ];
 #pragma unroll
         for (int j = 0; j < NQ; j++) {
-            qc[j] = QLDS ? 4 * (tid % TPR + TPR * j)
-                         : QN * (4 * (j / (QN / 4)) + g) + 4 * (j % (QN / 4));
+            qc[j] = 4 * (tid % TPR + TPR * j);
             qx[j] = *(const f4 *)(qsrc + 4 * (qat + (qc[j] < hd ? qc[j] : 0)));
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -465,8 +495,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         load_k(x);
         load_v(x);
 
-        u4 qr[QLDS ? 1 : KL][QLDS ? 1 : EB == 1 ? 2 : 1];
-        float qs2 = 1.0f, qmax = 0.0f;
+        float qmax = 0.0f;
 #pragma unroll
         for (int j = 0; j < NQ; j++) {
             /* (used as loaded: the compiler else loads only where it is kept, in
@@ -480,58 +509,54 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         }
         if constexpr (F32) {
 #pragma unroll
-            for (int j = 0; j < NQ; j++) {
-                if constexpr (QLDS)
-                    *(f4 *)&sQ[qrow][qc[j]] = qx[j];
-                else
-                    qr[j][0] = __builtin_bit_cast(u4, qx[j]);
-            }
+            for (int j = 0; j < NQ; j++)
+                *(f4 *)&sQ[qrow][qc[j]] = qx[j];
         } else {
-            /* the row's lanes: 32 side by side, or the four with the same n */
-            qmax = QLDS ? max_x16(max_row16(qmax)) : max_x32(max_x16(qmax));
+            qmax = max_x16(max_row16(qmax)); /* the row's 32 lanes */
             int ex = 0;
             if (qmax > 0.0f && qmax < INFINITY) {
                 frexpf(qmax, &ex);
                 ex = 14 - ex;
             }
-            const float up = ldexpf(1.0f, ex);
-            qs2 = ldexpf(1.0f, -ex);
+            const float up = ldexpf(1.0f, ex), neg1 = minus_one();
 #pragma unroll
             for (int j = 0; j < NQ; j++) {
-                h4 hi, lo;
+                h2 hi[2], lo[2];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    _Float16 y, z;
-                    split_hl(qx[j][e] * up, y, z);
-                    hi[e] = y;
-                    lo[e] = z;
-                }
-                if constexpr (QLDS) {
-                    *(h4 *)&sQ[2 * qrow][qc[j] / 2] = hi;
-                    *(h4 *)&sQ[2 * qrow + 1][qc[j] / 2] = lo;
-                } else {
-                    const uint2 y = __builtin_bit_cast(uint2, n & 1 ? lo : hi);
-                    qr[j / (QN / 4)][j % (QN / 4) / 2][2 * (j & 1)] = y.x;
-                    qr[j / (QN / 4)][j % (QN / 4) / 2][2 * (j & 1) + 1] = y.y;
+                for (int e = 0; e < 2; e++)
+                    split_hl2(qx[j][2 * e] * up, qx[j][2 * e + 1] * up, neg1, hi[e], lo[e]);
+                if (D >= 128 || qc[j] < D) {
+                    *(uint2 *)&sQ[2 * qrow][qc[j] / 2] = make_uint2(
+                        __builtin_bit_cast(uint32_t, hi[0]), __builtin_bit_cast(uint32_t, hi[1]));
+                    *(uint2 *)&sQ[2 * qrow + 1][qc[j] / 2] = make_uint2(
+                        __builtin_bit_cast(uint32_t, lo[0]), __builtin_bit_cast(uint32_t, lo[1]));
                 }
             }
-            if (QLDS && tid % TPR == 0)
-                sQs[qrow] = qs2;
+            if (tid % TPR == 0)
+                sQs[qrow] = ldexpf(1.0f, -ex);
         }
-        if constexpr (QLDS) {
-            __syncthreads();
-            if constexpr (!F32)
-                qs2 = sQs[n >> 1];
+        __syncthreads();
+        const float qs2 = (F32 ? 1.0f : sQs[n >> 1]) * A.scale * kLog2e;
+        constexpr int QO = EB == 1 ? 2 : 1; /* operands a K load */
+        auto q_place = [&](int i, int j, uint32_t place) {
+            return *(const u4 *)((const char *)&sQ[0][0] + place + 64 * QO * i + 16 * j);
+        };
+        const uint32_t qplace = n * S::QROW * 4 + 16 * QO * g;
+        u4 qr[QREG ? KL : 1][QREG ? QO : 1];
+        if constexpr (QREG) {
+#pragma unroll
+            for (int i = 0; i < KL; i++)
+#pragma unroll
+                for (int j = 0; j < QO; j++)
+                    qr[i][j] = q_place(i, j, qplace);
         }
-        qs2 = qs2 * A.scale * kLog2e;
-        /* operand j of K load i; `at`: the lane's place in LDS, unknown to the
-           compiler from unit to unit, so that the reads stay in the loop */
+        /* operand j of K load i; `place`: the lane's in LDS, unknown to the compiler
+           from unit to unit, so that the reads stay in the loop */
         auto q_operand = [&](int i, int j, uint32_t place) {
-            if constexpr (QLDS)
-                return *(const u4 *)((const char *)&sQ[0][0] + place + 64 * (EB == 1 ? 2 : 1) * i +
-                                     16 * j);
-            else
+            if constexpr (QREG)
                 return qr[i][j];
+            else
+                return q_place(i, j, place);
         };
 
         /* ---- the wave's positions ---- */
@@ -551,8 +576,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                 x = unit_of(u + 1);
             /* scores: lane holds positions 4 g + j of MFMA column n */
             f4 s{0, 0, 0, 0};
-            uint32_t place = n * S::QROW * 4 + 16 * (EB == 1 ? 2 : 1) * g;
-            if constexpr (QLDS)
+            uint32_t place = qplace;
+            if constexpr (!QREG)
                 asm volatile("" : "+v"(place));
 #pragma unroll
             for (int i = 0; i < KL; i++) {
@@ -667,6 +692,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         }
 
         /* ---- the waves joined ---- */
+        if constexpr (!QREG)
+            __syncthreads();
         l = sum_x32(sum_x16(l));
         if (__any(bad))
             l = NAN;
@@ -694,9 +721,10 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                     *(f4 *)&sO[w][r][16 * VN * c + VN * n + e] = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
             }
         __syncthreads();
-        const uint32_t c4 = hd / 4;      /* (hd: a multiple of 8) */
-        for (uint32_t t = tid; t < rows * c4; t += kPW * 64) {
-            const uint32_t r = t / c4, c = 4 * (t % c4);
+        for (uint32_t t = tid; t < rows * (D / 4); t += kPW * 64) {
+            const uint32_t r = t / (D / 4), c = 4 * (t % (D / 4));
+            if (c >= hd)
+                continue;
             const float mx = fmaxf(fmaxf(sM[0][r], sM[1][r]), fmaxf(sM[2][r], sM[3][r]));
             f4 y{0, 0, 0, 0};
             float sum = 0.0f;
@@ -859,10 +887,15 @@ __global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
 
 template <int T, int D> hipError_t launch_sel(const PagesArgs &a, hipStream_t s)
 {
-    if (a.sel)
-        hipLaunchKernelGGL((pages_kernel<T, D, true>), dim3(a.n_wg + (a.n_seqs > 64)), dim3(kPW * 64), 0, s, a);
+    const dim3 grid(a.rtiles, a.n_kv, a.runs + (a.n_seqs > 64)), block(kPW * 64);
+    if (a.sel && a.rtiles > 1)
+        hipLaunchKernelGGL((pages_kernel<T, D, true, true>), grid, block, 0, s, a);
+    else if (a.sel)
+        hipLaunchKernelGGL((pages_kernel<T, D, true, false>), grid, block, 0, s, a);
+    else if (a.rtiles > 1)
+        hipLaunchKernelGGL((pages_kernel<T, D, false, true>), grid, block, 0, s, a);
     else
-        hipLaunchKernelGGL((pages_kernel<T, D, false>), dim3(a.n_wg + (a.n_seqs > 64)), dim3(kPW * 64), 0, s, a);
+        hipLaunchKernelGGL((pages_kernel<T, D, false, false>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 

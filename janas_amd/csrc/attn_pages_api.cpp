@@ -112,7 +112,7 @@ int check_rows(const PagesGeom &g, const janas_attn_pages_call *c)
 /* the runs of a call and the bytes of their partials */
 struct Parts {
     uint32_t rtiles, share;
-    uint64_t n_wg, plan_bytes, ml_bytes, bytes;
+    uint64_t runs, plan_bytes, ml_bytes, bytes;
 };
 Parts parts_of(const PagesGeom &g, const janas_attn_pages *p)
 {
@@ -121,9 +121,8 @@ Parts parts_of(const PagesGeom &g, const janas_attn_pages *p)
     t.rtiles = (g.group + rows - 1) / rows;
     const uint32_t tiles = g.n_kv * t.rtiles;
     t.share = pages_share(p->kv_type, g.hd, g.cus, tiles);
-    const uint64_t runs = pages_runs(t.share, p->n_seqs, (uint64_t)p->max_pages * p->page / 16);
-    const uint64_t parts = (runs + p->n_seqs) * tiles * rows;
-    t.n_wg = runs * tiles;
+    t.runs = pages_runs(t.share, p->n_seqs, (uint64_t)p->max_pages * p->page / 16);
+    const uint64_t parts = (t.runs + p->n_seqs) * tiles * rows;
     t.plan_bytes = ((uint64_t)p->n_seqs * sizeof(uint2) + 255) / 256 * 256;
     t.ml_bytes = (parts * 2 * sizeof(float) + 255) / 256 * 256;
     t.bytes = t.plan_bytes + t.ml_bytes + parts * g.hd * sizeof(float);
@@ -302,7 +301,7 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
     const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + cols - 1) / cols);
     const uint64_t rows = c->row ? c->n_rows : p->n_seqs;
     const uint64_t blocks = rows * g.n_head * g.hd / JANAS_ATTN_QK;
-    if (std::max({t.n_wg + 1, merge_wg, c->out_q8k ? blocks : 0}) > kMostThreads / 256)
+    if (std::max({(t.runs + 1) * g.n_kv * t.rtiles, merge_wg, c->out_q8k ? blocks : 0}) > kMostThreads / 256)
         return JANAS_ATTN_ERANGE;
     if (c->work_bytes < t.bytes)
         return JANAS_ATTN_ERANGE;
@@ -337,7 +336,7 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
     s.q_stride = c->q_stride ? c->q_stride : g.n_head * g.hd;
     s.rtiles = t.rtiles;
     s.share = t.share;
-    s.n_wg = (uint32_t)t.n_wg;
+    s.runs = (uint32_t)t.runs;
     s.scale = g.scale;
     s.gate_mode = gate_mode;
     OnDevice on(p->dev);

@@ -553,7 +553,7 @@ def test_select(gpu, h, n_kv, hd, n_sel, first, last, window):
                 assert np.array_equal(want, got[i, kh]), (i, n, kh, want, got[i, kh])
 
 
-@pytest.mark.parametrize("nb", [1025, 2500, 8193])
+@pytest.mark.parametrize("nb", [513, 2500, 4097, 8193])
 def test_select_ties_and_many_blocks(gpu, nb):
     """Blocks of equal scores (the lower is taken), all of them equal, scores of
     both signs and zeros of both signs, over more blocks than threads, and than
