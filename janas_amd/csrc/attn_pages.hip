@@ -778,30 +778,33 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
 constexpr int kMBatch = 4;
 
 /*
- * A row's splits joined, COLS columns a workgroup: COLS / 4 lanes take a split
- * (a float4 each), so 1024 / COLS splits go at once, group i taking splits i, i
- * + groups, ... with a running maximum; the groups of a wave and then the waves
- * are joined in a fixed tree. Rows of one split are pages_kernel's; rows that
- * see nothing are written here: 0, or NaN where the length passes the table.
- * 32 columns where there are few rows (many splits each, and the device to
- * fill), 128 where there are many (pages_merge_cols).
+ * A row's partials joined, COLS columns a workgroup of WAVES waves: COLS / 4 lanes
+ * take a partial (a float4 each), so 256 / COLS x WAVES go at once, group i taking
+ * partials i, i + groups, ... with a running maximum; the groups of a wave and
+ * then the waves are joined in a fixed tree. Rows of one workgroup of
+ * pages_kernel's are written there; rows that see nothing are written here: 0, or
+ * NaN where the length passes the table.
+ *
+ * Bound by its launch and two dependent reads. 32 columns where there are few rows
+ * (many partials each, and the device to fill), 128 where there are many
+ * (pages_merge_cols), and one wave where a row has few partials.
  */
-template <int ROWS, int COLS>
-__global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
+template <int ROWS, int COLS, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void pages_merge_kernel(const PagesArgs A)
 {
-    constexpr uint32_t LANES = COLS / 4, GROUPS = 256 / LANES;
-    __shared__ float sM[4], sL[4];
-    __shared__ f4 sA[4][LANES];
+    constexpr uint32_t LANES = COLS / 4, GROUPS = WAVES * 64 / LANES;
+    __shared__ float sM[WAVES], sL[WAVES];
+    __shared__ f4 sA[WAVES][LANES];
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const uint32_t hd = A.hd, nd = (hd + COLS - 1) / COLS;
-    const uint32_t h = blockIdx.x / nd % A.n_head, si = blockIdx.x / nd / A.n_head;
-    const uint32_t col = blockIdx.x % nd * COLS + 4 * (lane % LANES);
+    const uint32_t hd = A.hd, h = blockIdx.y, si = blockIdx.z;
+    const uint32_t col = blockIdx.x * COLS + 4 * (lane % LANES);
     const uint2 plan = A.plan[si];
+    const uint32_t row = A.row ? A.row[si] : si;
     const uint32_t first = plan.x, count = plan.y;
     if (count == kNone || count == 1)
         return;
-    const size_t hr = (size_t)(A.row ? A.row[si] : si) * A.n_head + h;
+    const size_t hr = (size_t)row * A.n_head + h;
     if (count == 0) {
         const float z = A.len[si] > A.max_pages << A.page_log ? NAN : 0.0f;
         if (tid < LANES && col < hd)
@@ -811,6 +814,12 @@ __global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
     const uint32_t kvh = h / A.group, r = h % A.group;
     const uint32_t tiles = A.n_kv * A.rtiles, tile = kvh * A.rtiles + r / ROWS;
     const uint32_t at = col < hd ? col : 0;
+    /* the gate, asked for with the partials */
+    f4 sg{1, 1, 1, 1};
+    if (A.gate_mode == kGateElem)
+        sg = *(const f4 *)(A.gate + hr * hd + at);
+    else if (A.gate_mode == kGateHead)
+        sg[0] = sg[1] = sg[2] = sg[3] = A.gate[hr];
     float m = -INFINITY, l = 0.0f;
     f4 a{0, 0, 0, 0};
     for (uint32_t i0 = tid / LANES; i0 < count; i0 += GROUPS * kMBatch) {
@@ -842,7 +851,7 @@ __global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
                 a[c] = __builtin_fmaf(e, x[b][c], a[c]);
         }
     }
-    /* the wave's groups, then the 4 waves */
+    /* the wave's groups, then the waves */
     float mw = m;
 #pragma unroll
     for (int o = LANES; o < 64; o <<= 1)
@@ -857,30 +866,34 @@ __global__ __launch_bounds__(256) void pages_merge_kernel(const PagesArgs A)
         for (int c = 0; c < 4; c++)
             a[c] += __shfl_xor(a[c], o, 64);
     }
-    if (lane == 0) {
-        sM[w] = mw;
-        sL[w] = l;
+    float sum = l;
+    f4 y = a;
+    if constexpr (WAVES > 1) {
+        if (lane == 0) {
+            sM[w] = mw;
+            sL[w] = l;
+        }
+        if (lane < LANES)
+            sA[w][lane] = a;
+        __syncthreads();
+        if (tid >= LANES)
+            return;
+        float mx = sM[0];
+#pragma unroll
+        for (int i = 1; i < WAVES; i++)
+            mx = fmaxf(mx, sM[i]);
+        sum = 0.0f;
+        y = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) {
+            const float e = sM[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[i] - mx);
+            sum += e * sL[i];
+            y += e * sA[i][lane];
+        }
     }
-    if (lane < LANES)
-        sA[w][lane] = a;
-    __syncthreads();
     if (tid >= LANES || col >= hd)
         return;
-    const float mx = fmaxf(fmaxf(sM[0], sM[1]), fmaxf(sM[2], sM[3]));
-    float sum = 0.0f;
-    f4 y{0, 0, 0, 0};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float e = sM[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[i] - mx);
-        sum += e * sL[i];
-        y += e * sA[i][lane];
-    }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    f4 sg{1, 1, 1, 1};
-    if (A.gate_mode == kGateElem)
-        sg = *(const f4 *)(A.gate + hr * hd + col);
-    else if (A.gate_mode == kGateHead)
-        sg[0] = sg[1] = sg[2] = sg[3] = A.gate[hr];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         y[e] *= inv;
@@ -959,18 +972,28 @@ uint32_t pages_merge_cols(uint32_t n_seqs, uint32_t n_head, uint32_t hd)
     return hd > 32 && (uint64_t)n_seqs * n_head * ((hd + 127) / 128) >= kMergeFill ? 128 : 32;
 }
 
+template <int ROWS, int COLS> static void launch_merge_cols(const PagesArgs &a, hipStream_t s)
+{
+    const dim3 grid((a.hd + COLS - 1) / COLS, a.n_head, a.n_seqs);
+    /* a row's partials are about a sequence's share of the runs: a wave's batch
+       holds 4 x 256 / COLS of them */
+    if (a.share <= a.n_seqs * kMBatch * (256 / COLS))
+        hipLaunchKernelGGL((pages_merge_kernel<ROWS, COLS, 1>), grid, dim3(64), 0, s, a);
+    else
+        hipLaunchKernelGGL((pages_merge_kernel<ROWS, COLS, 4>), grid, dim3(256), 0, s, a);
+}
+
 hipError_t launch_pages_merge(int kv, const PagesArgs &a, hipStream_t s)
 {
-    const uint32_t cols = pages_merge_cols(a.n_seqs, a.n_head, a.hd);
-    const uint32_t n_wg = a.n_seqs * a.n_head * ((a.hd + cols - 1) / cols);
-    if (kv == kF32 && cols == 128)
-        hipLaunchKernelGGL((pages_merge_kernel<16, 128>), dim3(n_wg), dim3(256), 0, s, a);
+    const bool wide = pages_merge_cols(a.n_seqs, a.n_head, a.hd) == 128;
+    if (kv == kF32 && wide)
+        launch_merge_cols<16, 128>(a, s);
     else if (kv == kF32)
-        hipLaunchKernelGGL((pages_merge_kernel<16, 32>), dim3(n_wg), dim3(256), 0, s, a);
-    else if (cols == 128)
-        hipLaunchKernelGGL((pages_merge_kernel<8, 128>), dim3(n_wg), dim3(256), 0, s, a);
+        launch_merge_cols<16, 32>(a, s);
+    else if (wide)
+        launch_merge_cols<8, 128>(a, s);
     else
-        hipLaunchKernelGGL((pages_merge_kernel<8, 32>), dim3(n_wg), dim3(256), 0, s, a);
+        launch_merge_cols<8, 32>(a, s);
     return hipGetLastError();
 }
 

@@ -301,7 +301,8 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
     const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + cols - 1) / cols);
     const uint64_t rows = c->row ? c->n_rows : p->n_seqs;
     const uint64_t blocks = rows * g.n_head * g.hd / JANAS_ATTN_QK;
-    if (std::max({(t.runs + 1) * g.n_kv * t.rtiles, merge_wg, c->out_q8k ? blocks : 0}) > kMostThreads / 256)
+    if (std::max({(t.runs + 1) * g.n_kv * t.rtiles, merge_wg, c->out_q8k ? blocks : 0}) >
+            kMostThreads / 256 || g.n_head > 65535)
         return JANAS_ATTN_ERANGE;
     if (c->work_bytes < t.bytes)
         return JANAS_ATTN_ERANGE;
