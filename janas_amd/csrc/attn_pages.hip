@@ -194,13 +194,26 @@ template <int W> __device__ __forceinline__ uint32_t word(const typename Words<W
         return x[i];
 }
 
-/* waves a SIMD that an instance's registers leave room for, and with that the
-   workgroups a compute unit holds */
+/* waves a SIMD that an instance keeps its registers for, and with that the
+   workgroups a compute unit holds. f16 rows up to 128 stream faster with 3 than
+   with the 4 that fit (60 sequences at 4170 positions 165.4 -> 159.8 us; 2: 157.8,
+   but 100 sequences of up to 500 positions 29.9 -> 31.1); int8 rows, half as many
+   bytes in flight a wave, with 4 (32 to 8k 57.3, with 3 62.1) */
 constexpr int pages_waves(int kv, int d)
 {
     if (kv == kF32)
         return d <= 64 ? 4 : d <= 128 ? 2 : 1;
-    return d <= 64 ? 4 : d <= 128 ? (kv == kI16 ? 3 : 4) : d <= 256 ? (kv == kI8 ? 3 : 2) : 1;
+    return d <= 64 ? 4 : d <= 128 ? (kv == kI8 ? 4 : kv == kF16 ? 3 : 2) : d <= 256 ? (kv == kI8 ? 3 : 2) : 1;
+}
+
+/* units that a wave holds: two where rows of 64 bytes would leave too few bytes in
+   flight (32 sequences to 20k, 12 / 4 / 64 int8: 48.4 -> 40.3 us) or, at two waves
+   a SIMD, int16's many steps between loads (16 to 8k, 32 / 8 / 128: 55.7 -> 53.6).
+   Elsewhere the registers cost more than they bring: f32 at 256 59.6 -> 73.4, f16
+   and int16 at 64 a hundredth longer, no gain for f16 or int8 at 128 */
+constexpr int pages_buffers(int kv, int d)
+{
+    return (d == 64 && kv == kI8) || (d == 128 && kv == kI16) ? 2 : 1;
 }
 
 template <int T, int D> struct PS {
@@ -219,6 +232,7 @@ template <int T, int D> struct PS {
     static constexpr bool QREG = D < 256;
     static constexpr int QROW = F32 ? D + 4 : D / 2 + 4; /* words of an LDS row */
     static constexpr int WAVES = pages_waves(T, D);  /* a SIMD, by registers */
+    static constexpr int NB = pages_buffers(T, D);
 };
 
 template <bool KEEP, class V> __device__ __forceinline__ V load_once(const V *p)
@@ -283,7 +297,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
 {
     using S = PS<T, D>;
     constexpr int EB = S::EB, KL = S::KL, VN = S::VN, VU = S::VU, VW = S::VW, NT = S::NT;
-    constexpr int DP = S::DP, ROWS = S::ROWS;
+    constexpr int DP = S::DP, ROWS = S::ROWS, NB = S::NB;
     constexpr bool F32 = S::F32, SCALED = S::SCALED;
     typedef typename Words<VW>::T VT;
     /* the query's operands, and the waves' sums: from head size 256 on in the same
@@ -414,9 +428,12 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             return x;
         };
 
-        u4 kr[KL];
-        VT vr[4][VU];
-        f4 ks{1, 1, 1, 1}, vs{1, 1, 1, 1};
+        u4 kr[NB][KL];
+        VT vr[NB][4][VU];
+        f4 ks[NB], vs[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+            ks[i] = vs[i] = f4{1, 1, 1, 1};
         /* the lane's bytes of a K row, and its columns of a V row */
         uint32_t kat[KL], vat[VU];
         bool kback[KL];
@@ -435,17 +452,19 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             const uint32_t c = 16 * VN * u + VN * n;
             vat[u] = (c < hd ? c : 0) * EB;
         }
-        auto load_k = [&](const Unit &x) {
+        auto load_k = [&](const Unit &x, auto at) {
+            constexpr int B = decltype(at)::value;
             const char *const p = (const char *)A.k + x.row * rowb;
 #pragma unroll
             for (int i = 0; i < KL; i++)
-                kr[i] = load_once<MULTI>((const u4 *)(p + kat[i]));
+                kr[B][i] = load_once<MULTI>((const u4 *)(p + kat[i]));
             if constexpr (SCALED)
-                ks = *(const f4 *)(A.ks + x.row + 4 * g);
+                ks[B] = *(const f4 *)(A.ks + x.row + 4 * g);
         };
         /* value rows that are not in sight are read as the first or last one that is
            (they weigh 0, but what is there may be no number) */
-        auto load_v = [&](const Unit &x) {
+        auto load_v = [&](const Unit &x, auto at) {
+            constexpr int B = decltype(at)::value;
             const char *const p = (const char *)A.v + x.row * rowb;
             uint32_t r[4] = {4 * g * rowb, (4 * g + 1) * rowb, (4 * g + 2) * rowb, (4 * g + 3) * rowb};
             if (x.pos < sv.lo || x.pos + kUnit > sv.end) {
@@ -462,9 +481,9 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int u = 0; u < VU; u++)
-                    vr[j][u] = load_once<MULTI>((const VT *)(p + (r[j] + vat[u])));
+                    vr[B][j][u] = load_once<MULTI>((const VT *)(p + (r[j] + vat[u])));
             if constexpr (SCALED)
-                vs = *(const f4 *)(A.vs + x.row + 4 * g);
+                vs[B] = *(const f4 *)(A.vs + x.row + 4 * g);
         };
 
         /* ---- the query: MFMA column n's (row n / 2, plane n & 1; f32: row n) as the
@@ -492,8 +511,10 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         e0 = some >> upp_log;
         fetch(e0);
         Unit x = unit_of(some);
-        load_k(x);
-        load_v(x);
+        typedef std::integral_constant<int, 0> First;
+        typedef std::integral_constant<int, NB - 1> Second;
+        load_k(x, First());
+        load_v(x, First());
 
         float qmax = 0.0f;
 #pragma unroll
@@ -569,11 +590,19 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                                            within */
         float vup = 0.0f;               /* a weight's factor: 2^kUp over theirs */
         const float keep = lane & 1 ? -1.0f : -0.0f;
-        for (uint32_t u = first; u < last; u++) {
+        /* unit u from buffers `at`; with two, unit u + 1 is asked for whole before it,
+           into the others; with one, its keys once this one's are used, its values
+           after this one's */
+        auto unit = [&](uint32_t u, auto at, auto other) {
+            constexpr int B = decltype(at)::value;
             const Unit now = x;
             const bool more = u + 1 < last;
             if (more)
                 x = unit_of(u + 1);
+            if (NB == 2 && more) {
+                load_k(x, other);
+                load_v(x, other);
+            }
             /* scores: lane holds positions 4 g + j of MFMA column n */
             f4 s{0, 0, 0, 0};
             uint32_t place = qplace;
@@ -588,28 +617,28 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                     __builtin_amdgcn_sched_barrier(0);
                 const u4 q0 = q_operand(i, 0, place);
                 if constexpr (F32) {
-                    const f4 kf = __builtin_bit_cast(f4, kr[i]), qf = __builtin_bit_cast(f4, q0);
+                    const f4 kf = __builtin_bit_cast(f4, kr[B][i]), qf = __builtin_bit_cast(f4, q0);
 #pragma unroll
                     for (int e = 0; e < 4; e++)
                         s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s, 0, 0, 0);
                 } else if constexpr (T == kI8) {
-                    const u4 y = unit_fix(kr[i], kback[i]);
+                    const u4 y = unit_fix(kr[B][i], kback[i]);
                     s = mfma(i8_widen8(y.x, y.y), __builtin_bit_cast(h8, q0), s);
                     s = mfma(i8_widen8(y.z, y.w), __builtin_bit_cast(h8, q_operand(i, 1, place)), s);
                 } else if constexpr (T == kI16) {
                     h8 hi, lo;
-                    i16_planes8(kr[i].x, kr[i].y, kr[i].z, kr[i].w, hi, lo);
+                    i16_planes8(kr[B][i].x, kr[B][i].y, kr[B][i].z, kr[B][i].w, hi, lo);
                     s = mfma(hi, __builtin_bit_cast(h8, q0), s);
                     s = mfma(lo, __builtin_bit_cast(h8, q0), s);
                 } else {
-                    s = mfma(__builtin_bit_cast(h8, kr[i]), __builtin_bit_cast(h8, q0), s);
+                    s = mfma(__builtin_bit_cast(h8, kr[B][i]), __builtin_bit_cast(h8, q0), s);
                 }
             }
-            const f4 kz = ks;
-            if (more)
-                load_k(x);
+            const f4 kz = ks[B];
+            if (NB == 1 && more)
+                load_k(x, other);
             if (now.pos < sv.end && now.pos + kUnit > sv.lo) {
-                f4 vz = vs;
+                f4 vz = vs[B];
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if constexpr (!F32)
@@ -681,9 +710,9 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
 #pragma unroll
                             for (int j = 0; j < 4; j++)
                                 o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    pf[j], __uint_as_float(word<VW>(vr[j][c], e)), o[t], 0, 0, 0);
+                                    pf[j], __uint_as_float(word<VW>(vr[B][j][c], e)), o[t], 0, 0, 0);
                         } else {
-                            const VT v4[4] = {vr[0][c], vr[1][c], vr[2][c], vr[3][c]};
+                            const VT v4[4] = {vr[B][0][c], vr[B][1][c], vr[B][2][c], vr[B][3][c]};
                             h4 vb[DP];
                             value_operand<T, VW>(v4, e, vb);
 #pragma unroll
@@ -692,8 +721,13 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                         }
                     }
             }
-            if (more)
-                load_v(x);
+            if (NB == 1 && more)
+                load_v(x, other);
+        };
+        for (uint32_t u = first; u < last; u += NB) {
+            unit(u, First(), Second());
+            if (NB == 2 && u + 1 < last)
+                unit(u + 1, Second(), First());
         }
 
         /* ---- the waves joined ---- */
