@@ -464,7 +464,7 @@ struct janas_attn_rows {
  * janas_attn_q_prep bit for bit, in one launch. A row whose slot is
  * JANAS_ATTN_NONE or outside the pool, or whose position has no row of the
  * table (n_rot above 0), is left out: nothing of it is written, its q_out
- * row neither. Two rows with one slot are written in no order.
+ * row neither. What two rows with one slot leave there is not defined.
  */
 int janas_attn_pages_write(const struct janas_attn_pages *p,
                            const struct janas_attn_rows *r, void *stream);
@@ -474,8 +474,9 @@ int janas_attn_pages_write(const struct janas_attn_pages *p,
  * n_new[i] positions (a step's janas_attn_plan.granted; NULL: all its blocks)
  * are computed anew from the cached keys up to its length, as half floats
  * rounded outward and kept within +-65504 (NaN keys are passed over; a block
- * of nothing else gets 65504, -65504). max_new: the largest n_new, for the
- * launch's size only (0: not known).
+ * of nothing else gets 65504, -65504). A page that several sequences share gets
+ * those of one of them: the same ones where it is full. max_new: the largest
+ * n_new, for the launch's size only (0: not known).
  */
 int janas_attn_pages_bounds(const struct janas_attn_pages *p,
                             const uint32_t *n_new, uint32_t max_new,
@@ -484,8 +485,8 @@ int janas_attn_pages_bounds(const struct janas_attn_pages *p,
 /* A step's single tokens over the pool: the query of sequence i is row i of q
    and its output row i of out - or, with row and granted, row row[i], and
    sequences whose granted[i] is not 1 take no part (nothing of theirs is read
-   or written): janas_attn_plan's start and granted. row[i] at or past n_rows
-   takes no part either. */
+   or written): janas_attn_plan's start and granted. A row[i] at or past n_rows
+   takes no part either; those that do are distinct. Sequences may share pages. */
 struct janas_attn_pages_call {
     const float *q;          /* rows of n_head x head_dim */
     float *out;              /* the same, packed */
@@ -499,7 +500,8 @@ struct janas_attn_pages_call {
     void *work;              /* janas_attn_pages_work_bytes, 256-byte aligned;
                                 calls that may overlap need one each */
     size_t work_bytes;
-    void *out_q8k;           /* or NULL: as janas_attn_seq's */
+    void *out_q8k;           /* or NULL: as janas_attn_seq's, of every row of out
+                                (n_rows of them with row, else n_seqs) */
 };
 
 /* Device bytes that a janas_attn_pages_run or _select over p needs as work;

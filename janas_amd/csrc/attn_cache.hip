@@ -620,11 +620,10 @@ __global__ __launch_bounds__(256) void pages_rows16_kernel(const PagesRowArgs A)
 {
     __shared__ __attribute__((aligned(16))) float sR[kRowsWg][64 * NB];
     const uint32_t c = threadIdx.x % kRowLanes, w = threadIdx.x / kRowLanes;
-    const uint64_t id = (uint64_t)blockIdx.x * kRowsWg + w;
-    const uint32_t heads = A.n_kv + A.n_head;
-    if (id >= (uint64_t)A.n * heads)
+    const uint32_t id = blockIdx.x * kRowsWg + w, heads = A.n_kv + A.n_head;
+    if (id >= A.n * heads)
         return;
-    const uint32_t j = (uint32_t)(id / heads), r = (uint32_t)(id % heads);
+    const uint32_t j = id / heads, r = id % heads;
     const uint32_t hd = A.hd, half = A.n_rot / 2;
     const bool query = r >= A.n_kv;
     const float *const src = query ? A.q + (size_t)j * A.q_stride + (size_t)(r - A.n_kv) * hd
@@ -686,11 +685,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void pages_rows_kernel(const PagesR
     __shared__ float sK[kRowWaves][kMaxHd], sV[kRowWaves][kMaxHd];
     __shared__ float sS[kRowWaves];
     const uint32_t lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint64_t id = (uint64_t)blockIdx.x * kRowWaves + w;
-    const uint32_t heads = A.n_kv + A.n_head;
-    if (id >= (uint64_t)A.n * heads)
+    const uint32_t id = blockIdx.x * kRowWaves + w, heads = A.n_kv + A.n_head;
+    if (id >= A.n * heads)
         return;
-    const uint32_t j = (uint32_t)(id / heads), r = (uint32_t)(id % heads);
+    const uint32_t j = id / heads, r = id % heads;
     const uint32_t hd = A.hd, half = A.n_rot / 2;
     uint32_t slot, turn;
     if (!page_row(A, j, slot, turn))
@@ -813,13 +811,14 @@ template <int KV> static void pages_rows16(const PagesRowArgs &a, dim3 grid, hip
 
 hipError_t launch_pages_rows(const PagesRowArgs &a, hipStream_t s)
 {
-    const uint64_t rows = (uint64_t)a.n * (a.n_kv + a.n_head);
+    /* (below 2^26: janas_attn_pages_write) */
+    const uint32_t rows = a.n * (a.n_kv + a.n_head);
     const size_t word = 4 * elem_size(a.kv);
     if (a.hd % 4 == 0 && a.n_rot % 8 == 0 && a.k_stride % 4 == 0 && a.v_stride % 4 == 0 &&
         a.q_stride % 4 == 0 && aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.q, 16) &&
         aligned(a.q_out, 16) && aligned(a.k_norm, 16) && aligned(a.q_norm, 16) &&
         aligned(a.cs, 16) && aligned(a.sn, 16) && aligned(a.kc, word) && aligned(a.vc, word)) {
-        const dim3 grid((uint32_t)((rows + kRowsWg - 1) / kRowsWg));
+        const dim3 grid((rows + kRowsWg - 1) / kRowsWg);
         switch (a.kv) {
         case kI8:
             pages_rows16<kI8>(a, grid, s);
@@ -836,7 +835,7 @@ hipError_t launch_pages_rows(const PagesRowArgs &a, hipStream_t s)
         }
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(pages_rows_kernel, dim3((uint32_t)((rows + kRowWaves - 1) / kRowWaves)),
+    hipLaunchKernelGGL(pages_rows_kernel, dim3((rows + kRowWaves - 1) / kRowWaves),
                        dim3(64 * kRowWaves), 0, s, a);
     return hipGetLastError();
 }

@@ -338,6 +338,40 @@ def test_run_long_and_many(gpu, kv):
     check_run(pool, h, q, out, what="long and many")
 
 
+@pytest.mark.parametrize("kv,hd", [(KV_I8, 64), (KV_I8, 128), (KV_I16, 128), (KV_F16, 128),
+                                   (KV_F32, 64), (KV_F16, 256)])
+@pytest.mark.parametrize("picked", [False, True])
+def test_run_more_sequences_than_workgroups(gpu, kv, hd, picked):
+    """Workgroups that go from a sequence into the next, and on: more short
+    sequences than there are workgroups, among them empty and a long one."""
+    h, n_kv, page = 16, 8, 16
+    rng = np.random.default_rng([kv, hd])
+    lens = [int(x) for x in rng.integers(0, 90, 300)] + [3000] + [17] * 20
+    pool = ph.Pool(rng, kv, lens, page, n_kv, hd)
+    q = rng.standard_normal((len(lens), h, hd)).astype(np.float32)
+    sel = None
+    if picked:
+        sel = np.full((len(lens), n_kv, 4), ph.NONE, np.int32)
+        for i, n in enumerate(lens):
+            nb = ph.blocks(n, page)
+            for kh in range(n_kv):
+                m = min(nb, 4)
+                sel[i, kh, :m] = np.sort(rng.permutation(nb)[:m])
+    out = run_pages(gpu, pool, h, q, sel=sel, times=2)
+    check_run(pool, h, q, out, sel=sel, what="many sequences")
+
+
+def test_run_shared_pages(gpu):
+    """Sequences that begin with the same pages."""
+    h, n_kv, hd, page = 4, 2, 64, 16
+    rng = np.random.default_rng(12)
+    pool = ph.Pool(rng, KV_F16, [100, 77, 64], page, n_kv, hd)
+    pool.table[1, :3] = pool.table[0, :3]
+    pool.table[2, :4] = pool.table[0, :4]
+    q = rng.standard_normal((3, h, hd)).astype(np.float32)
+    check_run(pool, h, q, run_pages(gpu, pool, h, q), what="shared pages")
+
+
 @pytest.mark.parametrize("kv", [KV_I8, KV_I16], ids=NAMES.get)
 def test_run_value_scales_of_unlike_size(gpu, kv):
     """Value scales from 2^-60 to 2^20, growing, falling and mixed along a
