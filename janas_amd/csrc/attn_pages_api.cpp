@@ -255,6 +255,9 @@ extern "C" int janas_attn_pages_bounds(const struct janas_attn_pages *p,
     a.n_pages = p->n_pages;
     a.page_log = log2_of(p->page);
     a.kv = p->kv_type;
+    /* a workgroup each at least */
+    if ((uint64_t)p->n_seqs * p->n_kv > kMostThreads / 256)
+        return JANAS_ATTN_ERANGE;
     /* the blocks that max_new positions may touch; a workgroup goes on to
        further ones */
     uint64_t blocks = p->max_pages;

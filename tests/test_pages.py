@@ -97,6 +97,12 @@ def test_bounds_need_their_array():
                                             None) == jm.EINVAL
 
 
+def test_bounds_refuse_more_workgroups_than_a_launch_takes():
+    # 65535 sequences of 257 KV heads: 2^24 workgroups and more
+    p = pool(n_seqs=65535, n_kv=257)
+    assert at.lib().janas_attn_pages_bounds(ctypes.byref(p), A, 1, None) == jm.ERANGE
+
+
 def test_run_and_select_need_an_instance():
     L, p, c = at.lib(), ctypes.byref(pool()), at.PagesCall(q=A, out=A, work=A, work_bytes=1 << 30)
     assert L.janas_attn_pages_run(None, p, 0, ctypes.byref(c), None) == jm.EINVAL
