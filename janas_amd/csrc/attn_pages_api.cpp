@@ -109,6 +109,12 @@ int check_rows(const PagesGeom &g, const janas_attn_pages_call *c)
     return width > 0xFFFFFFFFu ? JANAS_ATTN_ERANGE : JANAS_ATTN_OK;
 }
 
+/* no rows, so that no sequence takes part */
+bool no_rows(const janas_attn_pages_call *c)
+{
+    return c && c->row && c->granted && c->n_rows == 0;
+}
+
 /* the runs of a call and the bytes of their partials */
 struct Parts {
     uint32_t rtiles, share;
@@ -180,6 +186,8 @@ extern "C" int janas_attn_pages_write(const struct janas_attn_pages *p,
     if (rc)
         return rc;
     const uint32_t hd = p->head_dim;
+    if (r && r->n == 0)
+        return JANAS_ATTN_OK; /* (an empty tensor has no address) */
     if (!r || !r->k || !r->v || !r->slot || r->n_rot % 2 || r->n_rot > hd ||
         (r->n_rot && (!r->cs || !r->sn || !r->pos || r->n_tab == 0)) ||
         (r->q && (!r->q_out || r->n_head == 0)))
@@ -191,8 +199,6 @@ extern "C" int janas_attn_pages_write(const struct janas_attn_pages *p,
         (r->q && r->q_stride && r->q_stride < qw) ||
         (r->q && r->q == r->q_out && r->q_stride && r->q_stride != qw))
         return JANAS_ATTN_EINVAL;
-    if (r->n == 0)
-        return JANAS_ATTN_OK;
     PagesRowArgs a;
     memset(&a, 0, sizeof a);
     a.k = r->k;
@@ -287,6 +293,8 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
     int rc = check_instance(a, p);
     if (rc)
         return rc;
+    if (no_rows(c))
+        return JANAS_ATTN_OK;
     const PagesGeom g = pages_geom(a);
     rc = check_rows(g, c);
     if (rc)
@@ -368,6 +376,8 @@ extern "C" int janas_attn_pages_select(struct janas_attn *a,
     int rc = check_instance(a, p);
     if (rc)
         return rc;
+    if (no_rows(c))
+        return JANAS_ATTN_OK;
     const PagesGeom g = pages_geom(a);
     rc = check_rows(g, c);
     if (rc)

@@ -434,6 +434,24 @@ def test_run_rows_that_take_part(gpu):
     assert (out[2:5] == 5.0).all()
 
 
+def test_calls_without_rows(gpu):
+    """A step in which nobody has a token: empty tensors, which have no address."""
+    rng = np.random.default_rng(43)
+    pool = ph.Pool(rng, KV_F16, [40, 20], 16, 1, 64)
+    g = OnGpu(pool, gpu, torch.zeros(pool.n_pages, 1, 2, 64, dtype=torch.float16, device=gpu))
+    zero = torch.zeros(2, dtype=torch.int32, device=gpu)
+    q = torch.zeros(0, 4, 64, device=gpu)
+    sel = torch.full((2, 1, 2), 7, dtype=torch.int32, device=gpu)
+    with jm.Attention(4, 1, 64, 64) as a:
+        part = dict(work=work_for(a, g.p, gpu), rows=zero, granted=zero)
+        a.run_pages(g.p, q, q.clone(), out_q8k=torch.zeros(0, dtype=torch.uint8, device=gpu), **part)
+        a.select(g.p, q, sel, **part)
+        at.pages_write(g.p, q[:, :1], q[:, :1], slot=zero[:0])
+        assert a.status() == 0
+    torch.cuda.synchronize()
+    assert bool((sel == 7).all())
+
+
 def test_run_strided_queries_and_q8k(gpu):
     h, n_kv, hd, page = 8, 2, 128, 64
     rng = np.random.default_rng(3)

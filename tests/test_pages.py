@@ -90,6 +90,9 @@ def test_write_of_no_rows_and_too_many():
     f = at.lib().janas_attn_pages_write
     assert f(ctypes.byref(pool()), ctypes.byref(rows(n=0)), None) == jm.OK
     assert f(ctypes.byref(pool()), ctypes.byref(rows(n=1 << 31)), None) == jm.ERANGE
+    # (an empty tensor has no address)
+    none = at.Rows(n=0, n_rot=64)
+    assert f(ctypes.byref(pool()), ctypes.byref(none), None) == jm.OK
 
 
 def test_bounds_need_their_array():
