@@ -518,7 +518,8 @@ size_t janas_attn_pages_work_bytes(const struct janas_attn *a,
  * and window; its scores are FLOAT's whatever its way, float-accurate over
  * every cache type: within 1e-5 of softmax-normalized outputs. A page outside
  * the pool, or a length past the table row, makes the row NaN; nothing outside
- * the arrays is read. How a sequence's positions are split depends on all
+ * the arrays is read. What is cached out of sight counts for nothing, NaN and
+ * infinities included; an infinite number in sight may make a row NaN. How a sequence's positions are split depends on all
  * the lengths of the call, so a row's last bits may differ from one batch to
  * another (the same call gives the same bits). JANAS_ATTN_ENOTSUP: a ring, head
  * sizes that janas_attn_run_dev_split refuses (f32 caches: above 256).
@@ -529,9 +530,9 @@ int janas_attn_pages_run(struct janas_attn *a, const struct janas_attn_pages *p,
 
 /*
  * The blocks each KV head's queries select, c->n_sel of them, into sel
- * (n_seqs x n_kv x n_sel; c->sel is not read): of the blocks in sight, the first `first` and the last `last` ones, and of the
- * others those with the largest scores, ascending, then JANAS_ATTN_NONE
- * where there are fewer. A block's score is the largest that any of the group's
+ * (n_seqs x n_kv x n_sel; c->sel is not read): of the blocks in sight, the
+ * first `first` and the last `last` ones, and of the others those with the
+ * largest scores, ascending, then JANAS_ATTN_NONE where there are fewer. A block's score is the largest that any of the group's
  * queries could give a key inside the block's bounds: max over the heads of
  * sum_d q_d x (q_d > 0 ? largest_d : smallest_d) (negated queries under a
  * negative scale), summed in double and rounded to float; of equal scores the

@@ -509,10 +509,17 @@ def _rows_of(x, what, shape):
 
 
 def _prepared(name, *args, keep):
-    """A call of an entry point as a function of no arguments."""
+    """A call of an entry point as a function of no arguments. The tensors among
+    what it keeps and its pool (keep[0]) are on one GPU."""
     f = getattr(lib(), name)
+    where = {str(x.device) for x in keep + keep[0].keep if hasattr(x, "device")}
+    if len(where) > 1:
+        raise ValueError(f"{name}: tensors on {', '.join(sorted(where))}")
+    host = not any(x.startswith("cuda") for x in where)
 
     def call():
+        if host:
+            raise ValueError(f"{name}: tensors in host memory")
         rc = f(*args)
         if rc != 0:
             raise AttnError(rc, name)

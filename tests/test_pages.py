@@ -146,6 +146,21 @@ def test_python_checks_tensors():
             f()
 
 
+def test_python_refuses_other_devices():
+    import torch
+    k = torch.zeros(8, 2, 16, 64, dtype=torch.float16)
+    x, slot = torch.zeros(5, 2, 64), torch.zeros(5, dtype=torch.int32)
+    t = dict(table=torch.zeros(3, 4, dtype=torch.int32), length=torch.zeros(3, dtype=torch.int32))
+    p = at.pages(k, k, kv_type=jm.KV_F16, **t)
+    with pytest.raises(ValueError, match="host memory"):
+        at.pages_write(p, x, x, slot=slot)
+    with pytest.raises(ValueError, match="cpu, meta"):
+        at.prepare_pages_write(p, x, x, slot=slot.to("meta"))
+    with pytest.raises(ValueError, match="cpu, meta"):
+        at.prepare_pages_bounds(at.pages(k, k, kv_type=jm.KV_F16, table=t["table"].to("meta"),
+                                         length=t["length"]))
+
+
 def test_plain_plan_keeps_pages_apart():
     """The restatement itself: over random steps every page is in one place -
     the free ones or one table row - and none is lost."""
