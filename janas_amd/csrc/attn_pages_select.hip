@@ -189,7 +189,13 @@ template <uint32_t N> __device__ __forceinline__ float largest16(const double *s
     return y;
 }
 
-constexpr uint32_t kScoreBlocks = 16;  /* blocks a workgroup at once, 16 lanes each */
+constexpr uint32_t kScoreRows = 16;    /* rows of 16 lanes a workgroup */
+/* rows of lanes that share a block where each takes `ht` of `heads` heads: 1, 2
+   or 4 */
+constexpr uint32_t score_share(uint32_t heads, uint32_t ht)
+{
+    return heads <= ht ? 1 : heads <= 2 * ht ? 2 : 4;
+}
 
 /*
  * A block's 16 lanes take 8 dimensions of every 128 each; HC: 128s of the head
@@ -197,10 +203,16 @@ constexpr uint32_t kScoreBlocks = 16;  /* blocks a workgroup at once, 16 lanes e
  * of its positive numbers, while the lanes go from block to block, the next
  * block's bounds asked for before this one's are used (their pages 16 blocks at
  * a time: a load less to wait for at each): a number and head are a
- * bit select, a conversion and a multiply-add. A group of more heads goes over
- * the blocks again.
+ * bit select, a conversion and a multiply-add. A larger group's heads go to up to
+ * four rows of lanes of one wave, which take a block together (bounds and selection
+ * of 16 / 2 heads of 256 over 5 x 375 blocks 20.9 -> 18.1 us against one row that
+ * goes over the blocks again, 32 / 1 of 128 over 4 x 940 with the attention 34.2 ->
+ * 28.6); what is above 16 / HC heads then goes over them again. Bound by those
+ * steps where blocks are many: 16 x 1000 blocks of 8 KV heads of 128 in 13 us, 2.6
+ * TB/s, of which vector instructions 9.5.
  */
-template <int HC> __global__ __launch_bounds__(256) void score_kernel(const SelectArgs A)
+template <int HC, uint32_t SHARE>
+__global__ __launch_bounds__(256) void score_kernel(const SelectArgs A)
 {
     constexpr uint32_t HT = 4 / HC;
     const uint32_t tid = threadIdx.x, si = blockIdx.z, kvh = blockIdx.y;
@@ -208,10 +220,11 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
     const Blocks bl = blocks_in_sight(A, sv);
     if (bl.n <= A.n_sel)
         return; /* all of them */
-    const uint32_t c = tid % 16, hd = A.hd, step = gridDim.x * kScoreBlocks;
-    const uint32_t j0 = blockIdx.x * kScoreBlocks + tid / 16;
+    const uint32_t c = tid % 16, hs = tid / 16 % SHARE, hd = A.hd;
+    const uint32_t blocks = kScoreRows / SHARE, step = gridDim.x * blocks;
+    const uint32_t j0 = blockIdx.x * blocks + tid / 16 / SHARE;
     if (j0 >= bl.n)
-        return; /* (a row of 16 lanes is whole or not there) */
+        return; /* (a block's rows of 16 lanes are all there or none) */
     const uint32_t *const table = A.table + (size_t)si * A.max_pages + bl.b0;
     float *const out = A.score + ((size_t)si * A.n_kv + kvh) * A.max_pages;
     bool in[HC];
@@ -236,7 +249,10 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
         }
     };
     fetch(j0);
-    for (uint32_t h0 = 0; h0 < A.group; h0 += HT) {
+    /* (a row of lanes past the group's heads takes the first ones again: the largest
+       stays what it is) */
+    for (uint32_t p0 = 0; p0 < A.group; p0 += HT * SHARE) {
+        const uint32_t mine = p0 + HT * hs, h0 = mine < A.group ? mine : p0;
         const float *const q =
             A.q + (size_t)sv.row * A.q_stride + ((size_t)kvh * A.group + h0) * hd;
         double x[HT][HC][8];
@@ -257,7 +273,7 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
                 }
             }
         h8 lo[HC], hi[HC];
-        if (h0 && (bl.n - 1 - j0) / step >= 16)
+        if (p0 && (bl.n - 1 - j0) / step >= 16)
             fetch(j0);
         boxes(0, lo, hi);
         for (uint32_t j = j0, k = 1; j < bl.n; j += step, k++) {
@@ -289,9 +305,13 @@ template <int HC> __global__ __launch_bounds__(256) void score_kernel(const Sele
                 /* (a head past the group: the first one again) */
                 sum[h] = h0 + h < A.group ? s : sum[0];
             }
-            const float best = largest16<HT>(sum, c);
-            if (c == 0)
-                out[j] = h0 == 0 ? best : fmaxf(best, out[j]);
+            float best = largest16<HT>(sum, c);
+            if constexpr (SHARE > 1)
+                best = fmaxf(best, __shfl_xor(best, 16, 64));
+            if constexpr (SHARE > 2)
+                best = fmaxf(best, __shfl_xor(best, 32, 64));
+            if (c == 0 && hs == 0)
+                out[j] = p0 == 0 ? best : fmaxf(best, out[j]);
         }
     }
 }
@@ -497,22 +517,35 @@ hipError_t launch_bounds(const BoundsArgs &a, hipStream_t s)
     return hipGetLastError();
 }
 
+template <int HC>
+static void launch_scores(const SelectArgs &a, uint32_t share, dim3 grid, hipStream_t s)
+{
+    if (share == 1)
+        hipLaunchKernelGGL((score_kernel<HC, 1>), grid, dim3(256), 0, s, a);
+    else if (share == 2)
+        hipLaunchKernelGGL((score_kernel<HC, 2>), grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((score_kernel<HC, 4>), grid, dim3(256), 0, s, a);
+}
+
 hipError_t launch_select(const SelectArgs &a, hipStream_t s)
 {
     /* as many workgroups as hold the table's blocks once, no more than fill the
        device (max_pages may be far above the lengths, and each workgroup makes
        its query first) */
     const uint32_t pairs = a.n_seqs * a.n_kv;
-    uint32_t x = (a.max_pages + kScoreBlocks - 1) / kScoreBlocks;
+    const uint32_t ht = a.hd <= 128 ? 4 : a.hd <= 256 ? 2 : 1;
+    const uint32_t share = score_share(a.group, ht), blocks = kScoreRows / share;
+    uint32_t x = (a.max_pages + blocks - 1) / blocks;
     const uint32_t most = pairs < 4 * a.cus ? 4 * a.cus / pairs : 1;
     x = x < most ? x : most;
     const dim3 grid(x, a.n_kv, a.n_seqs);
     if (a.hd <= 128)
-        hipLaunchKernelGGL(score_kernel<1>, grid, dim3(256), 0, s, a);
+        launch_scores<1>(a, share, grid, s);
     else if (a.hd <= 256)
-        hipLaunchKernelGGL(score_kernel<2>, grid, dim3(256), 0, s, a);
+        launch_scores<2>(a, share, grid, s);
     else
-        hipLaunchKernelGGL(score_kernel<4>, grid, dim3(256), 0, s, a);
+        launch_scores<4>(a, share, grid, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess)
         return e;

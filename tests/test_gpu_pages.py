@@ -584,7 +584,7 @@ def selected(gpu, pool, h, q, n_sel, first, last, *, window=0, boxes=None, scale
 
 
 @pytest.mark.parametrize("h,n_kv,hd", [(8, 2, 64), (32, 8, 128), (16, 2, 256), (7, 1, 72),
-                                       (34, 2, 512)])
+                                       (34, 2, 512), (40, 1, 128), (6, 2, 200)])
 @pytest.mark.parametrize("n_sel,first,last,window", [(1, 0, 0, 0), (5, 1, 2, 0), (4, 2, 2, 0),
                                                      (9, 0, 1, 500), (64, 1, 1, 0)])
 def test_select(gpu, h, n_kv, hd, n_sel, first, last, window):
