@@ -25,6 +25,7 @@ namespace janas {
 namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef int16_t s8 __attribute__((ext_vector_type(8)));
 typedef int8_t b8 __attribute__((ext_vector_type(8)));
@@ -49,52 +50,57 @@ __device__ __forceinline__ _Float16 outward(float x, bool up)
     return h;
 }
 
-/* 8 numbers of a cached row */
-__device__ __forceinline__ void load8(int kv, const void *p, size_t at, float z, float *x)
+/* 8 numbers of a cached row as they are, and as floats */
+template <int KV> struct Raw8;
+template <> struct Raw8<kI8> { typedef b8 T; };
+template <> struct Raw8<kI16> { typedef s8 T; };
+template <> struct Raw8<kF16> { typedef h8 T; };
+template <> struct Raw8<kF32> { typedef f8 T; };
+template <int KV> __device__ __forceinline__ typename Raw8<KV>::T load8(const void *p, size_t at)
 {
-    if (kv == kI8) {
-        const b8 r = *(const b8 *)((const int8_t *)p + at);
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            x[e] = (float)r[e] * z;
-    } else if (kv == kI16) {
-        const s8 r = *(const s8 *)((const int16_t *)p + at);
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            x[e] = (float)r[e] * z;
-    } else if (kv == kF16) {
-        const h8 r = *(const h8 *)((const _Float16 *)p + at);
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            x[e] = (float)r[e];
-    } else {
+    typedef typename Raw8<KV>::T T;
+    if constexpr (KV == kF32) { /* (aligned to 16 bytes) */
         const f4 a = *(const f4 *)((const float *)p + at), b = *(const f4 *)((const float *)p + at + 4);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x[e] = a[e];
-            x[4 + e] = b[e];
-        }
+        return T{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+        return *(const T *)((const char *)p + at * (sizeof(T) / 8));
     }
 }
 
-/*
- * A workgroup takes one block of a sequence and one KV head: its threads take 8
- * columns of every (256 / (hd / 8))-th row, then the rows' groups are joined in
- * LDS. Bound by reading the page once.
- */
-__global__ __launch_bounds__(256) void bounds_kernel(const BoundsArgs A)
+constexpr uint32_t kBoundRows = 4;     /* rows a thread asks for at once */
+constexpr uint32_t kBoundCols = 128;   /* columns a workgroup takes */
+__host__ __device__ constexpr uint32_t bound_slices(uint32_t hd)
 {
-    __shared__ float sLo[256][8], sHi[256][8];
+    return (hd + kBoundCols - 1) / kBoundCols;
+}
+
+/*
+ * A workgroup takes up to 128 columns of one block and KV head: its threads take 8
+ * of them in every (256 / (columns / 8))-th row, four rows asked for at once (one
+ * after the other: a page of 64 x 128 halves 5.1 -> 3.3 us, 5 x 6000 new positions
+ * of 2 x 256 9.0 -> 7.2 us, 4.3 TB/s; 8 at once no faster), then the rows' groups are
+ * joined in LDS. A workgroup for whole rows of 512 took 0.9 us longer. Bound by
+ * reading the page once, and for a decode's one block by its chain of reads - length,
+ * page, rows - and its launch.
+ */
+template <int KV> __global__ __launch_bounds__(256) void bounds_kernel(const BoundsArgs A)
+{
+    constexpr bool SCALED = KV == kI8 || KV == kI16;
+    __shared__ __attribute__((aligned(16))) float sLo[256][8], sHi[256][8];
     const uint32_t tid = threadIdx.x, si = blockIdx.z, kvh = blockIdx.y;
     const uint32_t page = 1u << A.page_log, cap = A.max_pages << A.page_log;
-    const uint32_t len = A.len[si] < cap ? A.len[si] : cap;
+    const uint32_t length = A.len[si], len = length < cap ? length : cap;
     uint32_t fresh = A.n_new ? A.n_new[si] : len;
     fresh = fresh < len ? fresh : len;
     if (fresh == 0)
         return;
-    const uint32_t b1 = (len + page - 1) >> A.page_log, units = A.hd / 8, groups = 256 / units;
+    const uint32_t b1 = (len + page - 1) >> A.page_log;
+    const uint32_t slices = bound_slices(A.hd), step = gridDim.x / slices;
+    const uint32_t c0 = blockIdx.x % slices * kBoundCols;
+    const uint32_t cols = A.hd - c0 < kBoundCols ? A.hd - c0 : kBoundCols;
+    const uint32_t units = cols / 8, groups = 256 / units;
     const uint32_t u = tid % units, rg = tid / units;
-    for (uint32_t b = ((len - fresh) >> A.page_log) + blockIdx.x; b < b1; b += gridDim.x) {
+    for (uint32_t b = ((len - fresh) >> A.page_log) + blockIdx.x / slices; b < b1; b += step) {
         const uint32_t pid = A.table[(size_t)si * A.max_pages + b];
         if (pid >= A.n_pages)
             continue;
@@ -107,28 +113,40 @@ __global__ __launch_bounds__(256) void bounds_kernel(const BoundsArgs A)
             hi[e] = -INFINITY;
         }
         if (rg < groups)
-            for (uint32_t r = rg; r < n; r += groups) {
-                float x[8];
-                load8(A.kv, A.k, (row0 + r) * A.hd + 8 * u, A.ks ? A.ks[row0 + r] : 1.0f, x);
+            for (uint32_t r0 = rg; r0 < n; r0 += kBoundRows * groups) {
+                typename Raw8<KV>::T x[kBoundRows];
+                float z[kBoundRows];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    lo[e] = fminf(lo[e], x[e]);
-                    hi[e] = fmaxf(hi[e], x[e]);
+                for (uint32_t i = 0; i < kBoundRows; i++) {
+                    /* (behind the last row: that one again) */
+                    const uint32_t r = r0 + i * groups < n ? r0 + i * groups : n - 1;
+                    x[i] = load8<KV>(A.k, (row0 + r) * A.hd + c0 + 8 * u);
+                    z[i] = SCALED ? A.ks[row0 + r] : 1.0f;
                 }
+#pragma unroll
+                for (uint32_t i = 0; i < kBoundRows; i++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float y = SCALED ? (float)x[i][e] * z[i] : (float)x[i][e];
+                        lo[e] = fminf(lo[e], y);
+                        hi[e] = fmaxf(hi[e], y);
+                    }
             }
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            sLo[tid][e] = lo[e];
-            sHi[tid][e] = hi[e];
+        for (int e = 0; e < 8; e += 4) {
+            *(f4 *)&sLo[tid][e] = f4{lo[e], lo[e + 1], lo[e + 2], lo[e + 3]};
+            *(f4 *)&sHi[tid][e] = f4{hi[e], hi[e + 1], hi[e + 2], hi[e + 3]};
         }
         __syncthreads();
-        for (uint32_t c = tid; c < A.hd; c += 256) {
+        if (tid < cols) {
+            const uint32_t c = tid;
             float l = INFINITY, h = -INFINITY;
+#pragma unroll 8
             for (uint32_t k = 0; k < groups; k++) {
                 l = fminf(l, sLo[k * units + c / 8][c % 8]);
                 h = fmaxf(h, sHi[k * units + c / 8][c % 8]);
             }
-            _Float16 *const o = A.bounds + ((size_t)pid * A.n_kv + kvh) * 2 * A.hd;
+            _Float16 *const o = A.bounds + ((size_t)pid * A.n_kv + kvh) * 2 * A.hd + c0;
             o[c] = outward(l, false);
             o[A.hd + c] = outward(h, true);
         }
@@ -513,7 +531,15 @@ __global__ __launch_bounds__(kPickThreads) void pick_kernel(const SelectArgs A)
 
 hipError_t launch_bounds(const BoundsArgs &a, hipStream_t s)
 {
-    hipLaunchKernelGGL(bounds_kernel, dim3(a.max_blocks, a.n_kv, a.n_seqs), dim3(256), 0, s, a);
+    const dim3 grid(a.max_blocks * bound_slices(a.hd), a.n_kv, a.n_seqs);
+    if (a.kv == kI8)
+        hipLaunchKernelGGL(bounds_kernel<kI8>, grid, dim3(256), 0, s, a);
+    else if (a.kv == kI16)
+        hipLaunchKernelGGL(bounds_kernel<kI16>, grid, dim3(256), 0, s, a);
+    else if (a.kv == kF16)
+        hipLaunchKernelGGL(bounds_kernel<kF16>, grid, dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL(bounds_kernel<kF32>, grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

@@ -525,7 +525,8 @@ def test_run_selected(gpu, kv, window):
 # ---- bounds and selection ---------------------------------------------------
 
 @pytest.mark.parametrize("kv", [KV_I8, KV_I16, KV_F16, KV_F32], ids=NAMES.get)
-@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 128), (512, 256), (72, 32)])
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 128), (512, 256), (72, 32), (200, 64),
+                                     (136, 16), (8, 64)])
 def test_bounds(gpu, kv, hd, page):
     n_kv = 2
     rng = np.random.default_rng([kv, hd])
