@@ -25,6 +25,7 @@ namespace janas {
 namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef float f8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef int16_t s8 __attribute__((ext_vector_type(8)));
@@ -362,6 +363,19 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t x)
     return x;
 }
 
+/* the largest over the wave, in lane 63 */
+__device__ __forceinline__ uint32_t max_wave(uint32_t x)
+{
+    auto up = [&](uint32_t y) { x = y > x ? y : x; };
+    up(shifted<0x111, 0xf>(x));
+    up(shifted<0x112, 0xf>(x));
+    up(shifted<0x114, 0xf>(x));
+    up(shifted<0x118, 0xf>(x));
+    up(shifted<0x142, 0xa>(x));
+    up(shifted<0x143, 0xc>(x));
+    return x;
+}
+
 /*
  * One workgroup a (sequence, KV head). Of the blocks that are not forced, the
  * `want`-th largest key is found 8 bits at a time, from the highest bit in which
@@ -376,8 +390,8 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t x)
 template <bool REG> __device__ void pick(const SelectArgs &A, const Blocks &bl, const float *score,
                                          uint32_t *sel)
 {
-    __shared__ uint32_t sHist[4][256], sFound[4][3];
-    __shared__ uint32_t sLow[kPickWaves], sHigh[kPickWaves];
+    __shared__ __attribute__((aligned(16))) uint32_t sHist[4][256];
+    __shared__ uint32_t sHigh[kPickWaves], sUnder[kPickWaves];
     __shared__ uint32_t sAbove[kPickWaves], sAt[kPickWaves];
     const uint32_t tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const uint32_t per = (bl.n + kPickThreads - 1) / kPickThreads, first = tid * per;
@@ -403,31 +417,32 @@ template <bool REG> __device__ void pick(const SelectArgs &A, const Blocks &bl, 
                     f(first + r, score_key(score[first + r]));
         }
     };
-    uint32_t low = 0xFFFFFFFFu, high = 0;
+    /* the largest key, and of the keys' complements (for the smallest) */
+    uint32_t high = 0, under = 0;
     each([&](uint32_t, uint32_t k) {
-        low = k < low ? k : low;
         high = k > high ? k : high;
+        under = ~k > under ? ~k : under;
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t a = __shfl_xor(low, o, 64), b = __shfl_xor(high, o, 64);
-        low = a < low ? a : low;
-        high = b > high ? b : high;
-    }
-    if (lane == 0) {
-        sLow[w] = low;
+    high = max_wave(high);
+    under = max_wave(under);
+    if (lane == 63) {
         sHigh[w] = high;
+        sUnder[w] = under;
     }
     for (uint32_t i = tid; i < 1024; i += kPickThreads)
         ((uint32_t *)sHist)[i] = 0;
     __syncthreads();
+    high = under = 0;
+#pragma unroll
     for (uint32_t i = 0; i < kPickWaves; i++) {
-        low = sLow[i] < low ? sLow[i] : low;
         high = sHigh[i] > high ? sHigh[i] : high;
+        under = sUnder[i] > under ? sUnder[i] : under;
     }
+    high = __builtin_amdgcn_readfirstlane(high);
+    const uint32_t differ = high ^ ~__builtin_amdgcn_readfirstlane(under);
     /* keys >= edge with the bits of `mask` are chosen, those equal to it in them
        until `want` is used up */
-    uint32_t want = A.n_sel - A.first - A.last, bits = low == high ? 0 : 32 - __builtin_clz(low ^ high);
+    uint32_t want = A.n_sel - A.first - A.last, bits = differ ? 32 - __builtin_clz(differ) : 0;
     uint32_t mask = bits == 32 ? 0 : 0xFFFFFFFFu << bits, edge = high & mask;
     for (int pass = 0; bits > 0 && want > 0; pass++) {
         const uint32_t shift = bits > 8 ? bits - 8 : 0, digits = (1u << (bits - shift)) - 1;
@@ -436,33 +451,22 @@ template <bool REG> __device__ void pick(const SelectArgs &A, const Blocks &bl, 
                 atomicAdd(&sHist[pass][k >> shift & digits], 1u);
         });
         __syncthreads();
-        /* the bin of the want-th from the top: one wave, 4 bins a lane from the
+        /* the bin of the want-th from the top, in every wave: 4 bins a lane from the
            top one down */
-        if (w == 0) {
-            uint32_t n[4], sum = 0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                n[e] = sHist[pass][255 - (4 * lane + e)];
-                sum += n[e];
-            }
-            const uint32_t s = scan_wave(sum);
-            uint32_t before = s - sum;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (before < want && want <= before + n[e]) {
-                    sFound[pass][0] = 255 - (4 * lane + e);
-                    sFound[pass][1] = want - before;
-                    sFound[pass][2] = n[e];
-                }
-                before += n[e];
-            }
-        }
-        __syncthreads();
+        const u4 n = *(const u4 *)&sHist[pass][252 - 4 * lane];
+        const uint32_t b1 = n[3], b2 = b1 + n[2], b3 = b2 + n[1], b4 = b3 + n[0];
+        const uint32_t upto = scan_wave(b4), left = want - (upto - b4);
+        const uint64_t hit = __ballot(want <= upto);
+        const uint32_t e = left <= b1 ? 0 : left <= b2 ? 1 : left <= b3 ? 2 : 3;
+        const uint32_t over = e == 0 ? 0 : e == 1 ? b1 : e == 2 ? b2 : b3;
+        const uint32_t l = (uint32_t)__builtin_ctzll(hit);
+        const uint32_t digit = __builtin_amdgcn_readlane(255 - (4 * lane + e), l);
+        const uint32_t in = __builtin_amdgcn_readlane(n[3 - e], l);
+        want = __builtin_amdgcn_readlane(left - over, l);
         bits = shift;
         mask |= digits << shift;
-        edge |= sFound[pass][0] << shift;
-        want = sFound[pass][1];
-        if (want == sFound[pass][2])
+        edge |= digit << shift;
+        if (want == in)
             break; /* all of that bin */
     }
     uint32_t above = 0, at = 0;
