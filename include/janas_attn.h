@@ -432,9 +432,9 @@ struct janas_attn_plan {
  * sequence is granted all of its tokens or none: none if they pass its table
  * row (max_pages x page) or the packed rows (max_tokens), and, from the first
  * one that finds too few free pages on, every sequence that needs one (those
- * that need none go on). Of pages a table row names twice, or a table with
- * entries outside the pool, nothing is checked here; no write leaves the
- * arrays. n_free above n_pages counts as n_pages.
+ * that need none go on). A page that two released rows name is returned twice;
+ * that, and table entries outside the pool, are not checked here; no write leaves
+ * the arrays. n_free above n_pages counts as n_pages.
  */
 int janas_attn_pages_plan(const struct janas_attn_pages *p,
                           const struct janas_attn_plan *s, void *stream);
@@ -514,15 +514,16 @@ size_t janas_attn_pages_work_bytes(const struct janas_attn *a,
  * position len - 1, sees positions max(0, len - window) .. len - 1, or those
  * of them in its KV head's selected blocks: of the first min(n_sel, blocks of
  * the sequence) entries, those below its block count (a block named twice
- * counts twice). A row that sees nothing is 0. The instance gives heads, scale
- * and window; its scores are FLOAT's whatever its way, float-accurate over
- * every cache type: within 1e-5 of softmax-normalized outputs. A page outside
- * the pool, or a length past the table row, makes the row NaN; nothing outside
- * the arrays is read. What is cached out of sight counts for nothing, NaN and
- * infinities included; an infinite number in sight may make a row NaN. How a sequence's positions are split depends on all
- * the lengths of the call, so a row's last bits may differ from one batch to
- * another (the same call gives the same bits). JANAS_ATTN_ENOTSUP: a ring, head
- * sizes that janas_attn_run_dev_split refuses (f32 caches: above 256).
+ * counts twice). A row that sees nothing is 0. The instance gives heads,
+ * scale and window; its scores are FLOAT's whatever its way, float-accurate
+ * over every cache type: within 1e-5 of softmax-normalized outputs. A page
+ * outside the pool, or a length past the table row, makes the row NaN;
+ * nothing outside the arrays is read. What is cached out of sight counts for
+ * nothing, NaN and infinities included; an infinite number in sight may make
+ * a row NaN. How a sequence's positions are split depends on all the lengths
+ * of the call, so a row's last bits may differ from one batch to another (the
+ * same call gives the same bits). JANAS_ATTN_ENOTSUP: a ring, head sizes that
+ * janas_attn_run_dev_split refuses (f32 caches: above 256).
  */
 int janas_attn_pages_run(struct janas_attn *a, const struct janas_attn_pages *p,
                          int gate_mode, const struct janas_attn_pages_call *c,
@@ -532,13 +533,13 @@ int janas_attn_pages_run(struct janas_attn *a, const struct janas_attn_pages *p,
  * The blocks each KV head's queries select, c->n_sel of them, into sel
  * (n_seqs x n_kv x n_sel; c->sel is not read): of the blocks in sight, the
  * first `first` and the last `last` ones, and of the others those with the
- * largest scores, ascending, then JANAS_ATTN_NONE where there are fewer. A block's score is the largest that any of the group's
- * queries could give a key inside the block's bounds: max over the heads of
- * sum_d q_d x (q_d > 0 ? largest_d : smallest_d) (negated queries under a
- * negative scale), summed in double and rounded to float; of equal scores the
- * lower block. Needs bounds, first + last <= n_sel, max_pages up to 2^20; c's
- * out, gate and out_q8k are not read. Rows of sequences that take no part stay
- * as they are.
+ * largest scores, ascending, then JANAS_ATTN_NONE where there are fewer. A
+ * block's score is the largest that any of the group's queries could give a
+ * key inside the block's bounds: max over the heads of sum_d q_d x (q_d > 0 ?
+ * largest_d : smallest_d) (negated queries under a negative scale), summed in
+ * double and rounded to float; of equal scores the lower block. Needs bounds,
+ * first + last <= n_sel, max_pages up to 2^20; c's out, gate and out_q8k are
+ * not read. Rows of sequences that take no part stay as they are.
  */
 int janas_attn_pages_select(struct janas_attn *a,
                             const struct janas_attn_pages *p,

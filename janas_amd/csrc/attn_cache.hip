@@ -613,7 +613,10 @@ __device__ __forceinline__ size_t page_at(const PagesRowArgs &A, uint32_t slot, 
 /*
  * rows16_kernel's rows into slots: of each token n_kv key and value rows, then
  * n_head query rows, 16 lanes a row. The slot and the position are read with
- * the row's numbers; only the rotation's table waits for the position.
+ * the row's numbers; only the rotation's table waits for the position. Read and
+ * written once, past the caches. Bound by memory: a batch of prompts of 16 / 2 / 256,
+ * f16, 189 MB in 40.5 us, 4.66 TB/s (with the caches 48.1; a copy 4.99); 64 tokens of
+ * 32 / 8 / 128 by the launch, 3.8 to 4.3 us.
  */
 template <int NB, int KV>
 __global__ __launch_bounds__(256) void pages_rows16_kernel(const PagesRowArgs A)

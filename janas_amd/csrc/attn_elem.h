@@ -208,6 +208,24 @@ __device__ __forceinline__ float from_x1(float a)
     return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(a), 0xB1, 0xf, 0xf, false));
 }
 
+/* the sum over the wave's lanes up to and with this one: DPP row_shr 1, 2, 4, 8
+   inside rows of 16, then row_bcast 15 and 31 across them (a lane without a
+   source adds 0) */
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t shifted(uint32_t x)
+{
+    return __builtin_amdgcn_update_dpp(0u, x, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x)
+{
+    x += shifted<0x111, 0xf>(x);
+    x += shifted<0x112, 0xf>(x);
+    x += shifted<0x114, 0xf>(x);
+    x += shifted<0x118, 0xf>(x);
+    x += shifted<0x142, 0xa>(x);
+    x += shifted<0x143, 0xc>(x);
+    return x;
+}
+
 /* log2(e), and the reference's weight cutoff e^-80 (attention.c:580) in
    powers of two: 80 / ln 2 */
 constexpr float kLog2e = 1.4426950408889634f;

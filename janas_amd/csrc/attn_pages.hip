@@ -28,6 +28,11 @@
  * row r in MFMA columns 2 r, 2 r + 1), cached integers and halves exact, f32
  * sums. An f32 cache takes f32 products (v_mfma_f32_16x16x4_f32) instead, 16
  * query rows a workgroup.
+ *
+ * Bound by memory where there is much to read - 60 sequences of 4170 positions, 32
+ * / 8 / 128 f16, in 160 us, 6.4 TB/s with the merge; 90000 positions of 16 / 2 / 512
+ * int16 in 76, 4.9 - and where there is little by the chain to the first row (length,
+ * table, row), some 4 us, and the two launches: 1000 positions of int8 8.4 us.
  */
 #include <math.h>
 #include <stdint.h>
@@ -69,22 +74,6 @@ __device__ __forceinline__ uint32_t seq_units(const PagesArgs &A, const SeqView 
     }
 }
 
-/* the sum over the lanes up to and with this one: row_shr 1, 2, 4, 8 inside
-   rows of 16, then row_bcast 15 and 31 across them */
-template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t shifted(uint32_t x)
-{
-    return __builtin_amdgcn_update_dpp(0u, x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t scan_wave(uint32_t x)
-{
-    x += shifted<0x111, 0xf>(x);
-    x += shifted<0x112, 0xf>(x);
-    x += shifted<0x114, 0xf>(x);
-    x += shifted<0x118, 0xf>(x);
-    x += shifted<0x142, 0xa>(x);
-    x += shifted<0x143, 0xc>(x);
-    return x;
-}
 __device__ __forceinline__ uint32_t sum_wave(uint32_t x)
 {
     return __builtin_amdgcn_readlane(scan_wave(x), 63);
@@ -203,7 +192,9 @@ constexpr int pages_waves(int kv, int d)
 {
     if (kv == kF32)
         return d <= 64 ? 4 : d <= 128 ? 2 : 1;
-    return d <= 64 ? 4 : d <= 128 ? (kv == kI8 ? 4 : kv == kF16 ? 3 : 2) : d <= 256 ? (kv == kI8 ? 3 : 2) : 1;
+    if (d <= 128)
+        return d <= 64 || kv == kI8 ? 4 : kv == kF16 ? 3 : 2;
+    return d > 256 ? 1 : kv == kI8 ? 3 : 2;
 }
 
 /* units that a wave holds: two where rows of 64 bytes would leave too few bytes in
@@ -466,7 +457,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         auto load_v = [&](const Unit &x, auto at) {
             constexpr int B = decltype(at)::value;
             const char *const p = (const char *)A.v + x.row * rowb;
-            uint32_t r[4] = {4 * g * rowb, (4 * g + 1) * rowb, (4 * g + 2) * rowb, (4 * g + 3) * rowb};
+            uint32_t r[4] = {4 * g * rowb, (4 * g + 1) * rowb, (4 * g + 2) * rowb,
+                             (4 * g + 3) * rowb};
             if (x.pos < sv.lo || x.pos + kUnit > sv.end) {
                 const uint32_t past = sv.end - 1 - x.pos, short_ = sv.lo - x.pos;
                 const uint32_t hi = x.pos < sv.end ? (past < 15 ? past : 15) : 0;
@@ -624,7 +616,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                 } else if constexpr (T == kI8) {
                     const u4 y = unit_fix(kr[B][i], kback[i]);
                     s = mfma(i8_widen8(y.x, y.y), __builtin_bit_cast(h8, q0), s);
-                    s = mfma(i8_widen8(y.z, y.w), __builtin_bit_cast(h8, q_operand(i, 1, place)), s);
+                    const u4 q1 = q_operand(i, 1, place);
+                    s = mfma(i8_widen8(y.z, y.w), __builtin_bit_cast(h8, q1), s);
                 } else if constexpr (T == kI16) {
                     h8 hi, lo;
                     i16_planes8(kr[B][i].x, kr[B][i].y, kr[B][i].z, kr[B][i].w, hi, lo);
@@ -710,14 +703,16 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
 #pragma unroll
                             for (int j = 0; j < 4; j++)
                                 o[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                                    pf[j], __uint_as_float(word<VW>(vr[B][j][c], e)), o[t], 0, 0, 0);
+                                    pf[j], __uint_as_float(word<VW>(vr[B][j][c], e)), o[t],
+                                    0, 0, 0);
                         } else {
                             const VT v4[4] = {vr[B][0][c], vr[B][1][c], vr[B][2][c], vr[B][3][c]};
                             h4 vb[DP];
                             value_operand<T, VW>(v4, e, vb);
 #pragma unroll
                             for (int d = 0; d < DP; d++)
-                                o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, vb[d], o[t], 0, 0, 0);
+                                o[t] = __builtin_amdgcn_mfma_f32_16x16x16f16(pa, vb[d], o[t],
+                                                                             0, 0, 0);
                         }
                     }
             }
@@ -757,7 +752,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                     y[e] = F32 ? o[c * VN + e][i] : o[c * VN + e][2 * i] + o[c * VN + e][2 * i + 1];
 #pragma unroll
                 for (int e = 0; e < VN; e += 4)
-                    *(f4 *)&sO[w][r][16 * VN * c + VN * n + e] = f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+                    *(f4 *)&sO[w][r][16 * VN * c + VN * n + e] =
+                        f4{y[e], y[e + 1], y[e + 2], y[e + 3]};
             }
         __syncthreads();
         for (uint32_t t = tid; t < rows * (D / 4); t += kPW * 64) {
@@ -769,7 +765,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < kPW; i++) {
-                const float f = sM[i][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sM[i][r] - mx);
+                const float mi = sM[i][r];
+                const float f = mi == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mi - mx);
                 sum += f * sL[i][r];
                 const f4 x = *(const f4 *)&sO[i][r][c];
                 const float fo = f * sE[i];
@@ -819,7 +816,7 @@ constexpr int kMBatch = 4;
  * pages_kernel's are written there; rows that see nothing are written here: 0, or
  * NaN where the length passes the table.
  *
- * Bound by its launch and two dependent reads. 32 columns where there are few rows
+ * Bound by its launch and two dependent reads: 3.5 to 4.7 us. 32 columns where there are few rows
  * (many partials each, and the device to fill), 128 where there are many
  * (pages_merge_cols), and one wave where a row has few partials.
  */

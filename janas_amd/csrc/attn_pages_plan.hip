@@ -10,33 +10,18 @@
  * launch. A large step's tokens and pages go to a second kernel, a thread each,
  * which finds a token's sequence in the first rows by halving.
  *
- * Bound by its launches: a step of 48 sequences moves 2 KB.
+ * Bound by its launches: a step of 48 sequences moves 2 KB (3.0 to 4.0 us, as an
+ * empty kernel), one of 46 prompts and 44 000 tokens 0.56 MB (4.8 + 3.8 us).
  */
 #include <stdint.h>
 
 #include <hip/hip_runtime.h>
 
+#include "attn_elem.h"
 #include "attn_pages.h"
 
 namespace janas {
 namespace {
-
-/* the sum over the lanes up to and with this one (row_shr 1, 2, 4, 8, then
-   row_bcast 15 and 31) */
-template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t shifted(uint32_t x)
-{
-    return __builtin_amdgcn_update_dpp(0u, x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t scan_wave(uint32_t x)
-{
-    x += shifted<0x111, 0xf>(x);
-    x += shifted<0x112, 0xf>(x);
-    x += shifted<0x114, 0xf>(x);
-    x += shifted<0x118, 0xf>(x);
-    x += shifted<0x142, 0xa>(x);
-    x += shifted<0x143, 0xc>(x);
-    return x;
-}
 
 /* the sum of x (below 2^32) over the threads before this one; total: over all */
 template <uint32_t WAVES>
@@ -170,7 +155,8 @@ __global__ __launch_bounds__(WAVES * 64) void plan_kernel(const PlanArgs A)
         const uint64_t first = tok + scan_group<WAVES>(add, sScan, all_tok);
         const bool fits = (uint64_t)old + add <= room && first + add <= A.max_tokens;
         const uint32_t have = (uint32_t)blocks_of(old, A.page_log);
-        const uint32_t need = fits ? (uint32_t)blocks_of((uint64_t)old + add, A.page_log) - have : 0;
+        const uint32_t held = (uint32_t)blocks_of((uint64_t)old + add, A.page_log);
+        const uint32_t need = fits ? held - have : 0;
         const uint64_t before = asked + scan_group<WAVES>(need, sScan, all_need);
         const bool ok = fits && (need == 0 || before + need <= top);
         /* the pages taken up to here: once a sequence found too few, none */

@@ -17,6 +17,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include "attn_elem.h"
 #include "attn_pages.h"
 
 #pragma clang fp contract(off)
@@ -61,7 +62,8 @@ template <int KV> __device__ __forceinline__ typename Raw8<KV>::T load8(const vo
 {
     typedef typename Raw8<KV>::T T;
     if constexpr (KV == kF32) { /* (aligned to 16 bytes) */
-        const f4 a = *(const f4 *)((const float *)p + at), b = *(const f4 *)((const float *)p + at + 4);
+        const float *const x = (const float *)p + at;
+        const f4 a = *(const f4 *)x, b = *(const f4 *)(x + 4);
         return T{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     } else {
         return *(const T *)((const char *)p + at * (sizeof(T) / 8));
@@ -227,8 +229,8 @@ constexpr uint32_t score_share(uint32_t heads, uint32_t ht)
  * of 16 / 2 heads of 256 over 5 x 375 blocks 20.9 -> 18.1 us against one row that
  * goes over the blocks again, 32 / 1 of 128 over 4 x 940 with the attention 34.2 ->
  * 28.6); what is above 16 / HC heads then goes over them again. Bound by those
- * steps where blocks are many: 16 x 1000 blocks of 8 KV heads of 128 in 13 us, 2.6
- * TB/s, of which vector instructions 9.5.
+ * steps where blocks are many: 8673 blocks of 8 KV heads of 128 in 13.5 us, 2.6 TB/s,
+ * of which vector instructions 9.5.
  */
 template <int HC, uint32_t SHARE>
 __global__ __launch_bounds__(256) void score_kernel(const SelectArgs A)
@@ -346,23 +348,6 @@ __device__ __forceinline__ uint32_t score_key(float x)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-/* the sum over the lanes up to and with this one (as scan_wave in
-   attn_pages.hip) */
-template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t shifted(uint32_t x)
-{
-    return __builtin_amdgcn_update_dpp(0u, x, CTRL, ROWS, 0xf, false);
-}
-__device__ __forceinline__ uint32_t scan_wave(uint32_t x)
-{
-    x += shifted<0x111, 0xf>(x);
-    x += shifted<0x112, 0xf>(x);
-    x += shifted<0x114, 0xf>(x);
-    x += shifted<0x118, 0xf>(x);
-    x += shifted<0x142, 0xa>(x);
-    x += shifted<0x143, 0xc>(x);
-    return x;
-}
-
 /* the largest over the wave, in lane 63 */
 __device__ __forceinline__ uint32_t max_wave(uint32_t x)
 {
@@ -384,8 +369,8 @@ __device__ __forceinline__ uint32_t max_wave(uint32_t x)
  * each thread counts its own chosen blocks - neighbours, so that a scan of the
  * counts puts them in order - and writes them. REG: the thread's keys stay in
  * registers; else they are read again at each step. Bound by its chain of steps:
- * 512 threads measured best (2000 blocks: a selection's calls 28.4 us, with 256
- * threads 29.5, with 1024 28.8).
+ * 512 threads measured best (2000 blocks, with bounds, scores and the attention: 25.6
+ * us, with 256 threads 26.5, with 1024 26.0; this kernel alone 6.3 under the tracer).
  */
 template <bool REG> __device__ void pick(const SelectArgs &A, const Blocks &bl, const float *score,
                                          uint32_t *sel)

@@ -444,7 +444,8 @@ def test_calls_without_rows(gpu):
     sel = torch.full((2, 1, 2), 7, dtype=torch.int32, device=gpu)
     with jm.Attention(4, 1, 64, 64) as a:
         part = dict(work=work_for(a, g.p, gpu), rows=zero, granted=zero)
-        a.run_pages(g.p, q, q.clone(), out_q8k=torch.zeros(0, dtype=torch.uint8, device=gpu), **part)
+        blocks = torch.zeros(0, dtype=torch.uint8, device=gpu)
+        a.run_pages(g.p, q, q.clone(), out_q8k=blocks, **part)
         a.select(g.p, q, sel, **part)
         at.pages_write(g.p, q[:, :1], q[:, :1], slot=zero[:0])
         assert a.status() == 0
@@ -525,8 +526,8 @@ def test_run_selected(gpu, kv, window):
 # ---- bounds and selection ---------------------------------------------------
 
 @pytest.mark.parametrize("kv", [KV_I8, KV_I16, KV_F16, KV_F32], ids=NAMES.get)
-@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 128), (512, 256), (72, 32), (200, 64),
-                                     (136, 16), (8, 64)])
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64), (256, 128), (512, 256), (72, 32),
+                                     (200, 64), (136, 16), (8, 64)])
 def test_bounds(gpu, kv, hd, page):
     n_kv = 2
     rng = np.random.default_rng([kv, hd])
