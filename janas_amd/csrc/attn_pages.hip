@@ -290,6 +290,10 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
     constexpr int EB = S::EB, KL = S::KL, VN = S::VN, VU = S::VU, VW = S::VW, NT = S::NT;
     constexpr int DP = S::DP, ROWS = S::ROWS, NB = S::NB;
     constexpr bool F32 = S::F32, SCALED = S::SCALED;
+    /* where a K row's loads lie is found anew for each unit, not kept in 16 registers
+       (16 x 4000 positions of 16 / 4 / 256: 58.7 -> 57.8 us; not for int16 at 512,
+       76.0 -> 77.9, whose registers hold) */
+    constexpr bool LEAN = F32 && D == 256;
     typedef typename Words<VW>::T VT;
     /* the query's operands, and the waves' sums: from head size 256 on in the same
        place */
@@ -446,9 +450,18 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         auto load_k = [&](const Unit &x, auto at) {
             constexpr int B = decltype(at)::value;
             const char *const p = (const char *)A.k + x.row * rowb;
+            uint32_t kb = 16 * g;
+            if constexpr (LEAN)
+                asm volatile("" : "+v"(kb));
 #pragma unroll
-            for (int i = 0; i < KL; i++)
-                kr[B][i] = load_once<MULTI>((const u4 *)(p + kat[i]));
+            for (int i = 0; i < KL; i++) {
+                uint32_t to = kat[i];
+                if constexpr (LEAN) {
+                    to = 64 * i + kb;
+                    to = (to < rowb ? to : 0) + n * rowb;
+                }
+                kr[B][i] = load_once<MULTI>((const u4 *)(p + to));
+            }
             if constexpr (SCALED)
                 ks[B] = *(const f4 *)(A.ks + x.row + 4 * g);
         };
