@@ -187,14 +187,17 @@ template <int W> __device__ __forceinline__ uint32_t word(const typename Words<W
    workgroups a compute unit holds. f16 rows up to 128 stream faster with 3 than
    with the 4 that fit (60 sequences at 4170 positions 165.4 -> 159.8 us; 2: 157.8,
    but 100 sequences of up to 500 positions 29.9 -> 31.1); int8 rows, half as many
-   bytes in flight a wave, with 4 (32 to 8k 57.3, with 3 62.1) */
+   bytes in flight a wave, with 4 (32 to 8k 57.3, with 3 62.1), and at 512 with 2
+   (60 000 positions, 16 / 2 heads: 41.5 -> 34.5 against 1) */
 constexpr int pages_waves(int kv, int d)
 {
     if (kv == kF32)
         return d <= 64 ? 4 : d <= 128 ? 2 : 1;
     if (d <= 128)
         return d <= 64 || kv == kI8 ? 4 : kv == kF16 ? 3 : 2;
-    return d > 256 ? 1 : kv == kI8 ? 3 : 2;
+    if (d <= 256)
+        return kv == kI8 ? 3 : 2;
+    return kv == kI8 ? 2 : 1;
 }
 
 /* units that a wave holds: two where rows of 64 bytes would leave too few bytes in
@@ -290,10 +293,11 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
     constexpr int EB = S::EB, KL = S::KL, VN = S::VN, VU = S::VU, VW = S::VW, NT = S::NT;
     constexpr int DP = S::DP, ROWS = S::ROWS, NB = S::NB;
     constexpr bool F32 = S::F32, SCALED = S::SCALED;
-    /* where a K row's loads lie is found anew for each unit, not kept in 16 registers
-       (16 x 4000 positions of 16 / 4 / 256: 58.7 -> 57.8 us; not for int16 at 512,
-       76.0 -> 77.9, whose registers hold) */
-    constexpr bool LEAN = F32 && D == 256;
+    /* where a K row's loads lie is found anew for each unit, not kept in up to 16
+       registers (f32, 16 x 4000 positions of 16 / 4 / 256: 58.7 -> 57.8 us; int8 at
+       512 has room for a second wave a SIMD with it; not for int16 at 512, 76.0 ->
+       77.9, whose registers hold) */
+    constexpr bool LEAN = (F32 && D == 256) || (T == kI8 && D == 512);
     typedef typename Words<VW>::T VT;
     /* the query's operands, and the waves' sums: from head size 256 on in the same
        place */
@@ -457,8 +461,9 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             for (int i = 0; i < KL; i++) {
                 uint32_t to = kat[i];
                 if constexpr (LEAN) {
+                    bool back;
                     to = 64 * i + kb;
-                    to = (to < rowb ? to : 0) + n * rowb;
+                    to = (EB == 1 ? unit_at(to, rowb, back) : to < rowb ? to : 0) + n * rowb;
                 }
                 kr[B][i] = load_once<MULTI>((const u4 *)(p + to));
             }
@@ -617,8 +622,8 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             for (int i = 0; i < KL; i++) {
                 /* (else the query's reads for all of them are made first, in
                    registers that are not there: 90k positions of int16, 80.5 ->
-                   77.7 us) */
-                if (D > 256 && i % 4 == 0)
+                   77.7 us; int8 holds those of one load with two waves a SIMD) */
+                if (D > 256 && (T == kI8 || i % 4 == 0))
                     __builtin_amdgcn_sched_barrier(0);
                 const u4 q0 = q_operand(i, 0, place);
                 if constexpr (F32) {
