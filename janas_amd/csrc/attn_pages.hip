@@ -500,7 +500,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
            B operand of each K load. Planes: scaled by 2^ex so that the row's
            largest lies in [2^13, 2^14). The workgroup makes them once, 256 / ROWS
            lanes a row, words of four, through LDS; asked for first, made when the
-           first unit has been asked for: one round trip for the query and the
+           first unit's keys have been asked for: one round trip for the query and the
            table, one for the unit ---- */
         constexpr int TPR = kPW * 64 / ROWS, NQ = (D + 4 * TPR - 1) / (4 * TPR);
         const uint32_t qrow = tid / TPR;
@@ -524,7 +524,6 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
         typedef std::integral_constant<int, 0> First;
         typedef std::integral_constant<int, NB - 1> Second;
         load_k(x, First());
-        load_v(x, First());
 
         float qmax = 0.0f;
 #pragma unroll
@@ -566,7 +565,15 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             if (tid % TPR == 0)
                 sQs[qrow] = ldexpf(1.0f, -ex);
         }
+        /* (its values once the planes are made, which wait for the query alone; against
+           with the keys: 90k positions of 16 / 2 / 512 int16 76.1 -> 73.7 us, 16 to 16k
+           of 16 / 2 / 256 int8 36.2 -> 35.0; f32's, of which the planes are no more than
+           a copy, before the others are waited for: 16 to 4k of 256 57.2, after 59.7) */
+        if constexpr (F32)
+            load_v(x, First());
         __syncthreads();
+        if constexpr (!F32)
+            load_v(x, First());
         const float qs2 = (F32 ? 1.0f : sQs[n >> 1]) * A.scale * kLog2e;
         constexpr int QO = EB == 1 ? 2 : 1; /* operands a K load */
         auto q_place = [&](int i, int j, uint32_t place) {
