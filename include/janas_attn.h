@@ -15,7 +15,9 @@
  * Part 2 extends it for callers that keep everything on the device: f16
  * and f32 caches besides int8 / int16, any number of tokens a call, several
  * sequences a call (each its own cache), the output gate fused, and an
- * asynchronous stream. It has no counterpart in the reference header.
+ * asynchronous stream. It has no counterpart in the reference header. Part 3 is
+ * the cache around the attention (writes, shift, state rows), Part 4 a cache in
+ * pages that many sequences share.
  *
  * Errors. janas_attn_create returns NULL on a geometry the reference
  * rejects (attention.c:998-1000) or when the device cannot be used.
@@ -27,8 +29,9 @@
  * 705). By default janas_attn_run then aborts, since the library has no CPU
  * path; after janas_attn_set_abort(a, 0) it returns instead, with a host
  * output filled with NaN, so the engine can check the status and fall back
- * to its own attention. The Part 2 entry points return 0 or a negative
- * JANAS_ATTN_E* code, never abort, and remember device failures too.
+ * to its own attention. The entry points of Parts 2 to 4 return 0 or a negative
+ * JANAS_ATTN_E* code and never abort; those that take an instance remember device
+ * failures too.
  */
 #ifndef JANAS_ATTN_HIP_H
 #define JANAS_ATTN_HIP_H

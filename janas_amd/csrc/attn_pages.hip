@@ -31,8 +31,8 @@
  *
  * Bound by memory where there is much to read - 60 sequences of 4170 positions, 32
  * / 8 / 128 f16, in 160 us, 6.4 TB/s with the merge; 90000 positions of 16 / 2 / 512
- * int16 in 76, 4.9 - and where there is little by the chain to the first row (length,
- * table, row), some 4 us, and the two launches: 1000 positions of int8 8.4 us.
+ * int16 in 73.5, 5.0 - and where there is little by the chain to the first row (length,
+ * table, row), some 4 us, and the two launches: 1000 positions of int8 8.2 us.
  */
 #include <math.h>
 #include <stdint.h>
