@@ -230,9 +230,12 @@ def _ints(x):
 
 
 def _quant(x, kv):
-    """Rows at 8 or 16 bits with a scale each, as the cache write makes them."""
-    top = TOP[kv]
+    """Rows at 8 or 16 bits with a scale each, as the cache write makes them:
+    the multiplier and the scale are one quotient each, rounded once. (A number
+    over a tensor is the number times the reciprocal, rounded twice, and so on
+    the GPU is a tensor over a number: quotients of two tensors.)"""
     mx = x.abs().amax(-1)
+    top = torch.full_like(mx, TOP[kv])
     inv = torch.where(mx > 0, top / mx, torch.zeros_like(mx))
     return torch.round(x * inv[..., None]).to(DTYPE[kv]), mx / top
 
@@ -665,12 +668,23 @@ def _exact_write(s):
     for name, z in (("k", "ks"), ("v", "vs")):
         x = new[name]
         if c["kv"] in TOP:
-            # whole numbers beside their scale: a tie's side is the 32-bit
-            # arithmetic's
+            top = torch.tensor(TOP[c["kv"]], dtype=torch.float64, device=DEV)
+            mx = x.abs().amax(-1)
             full = p[z].double().transpose(1, 2).contiguous()
-            full[page, off] = x.abs().amax(-1) / TOP[c["kv"]]
+            full[page, off] = mx / top
             scales.append(full.transpose(1, 2))
-            res.append(None)
+            if name == "k":
+                # whole numbers beside their scale: a tie's side is the 32-bit
+                # arithmetic's, of the norm and the rotation too
+                res.append(None)
+                continue
+            # the values' are the rule's own: a quotient and a product, each
+            # rounded once to 32 bits (from 64, where either is near enough
+            # exact), and the nearest whole number
+            inv = torch.where(mx > 0, torch.full_like(mx, TOP[c["kv"]]) / mx, 0.0).float()
+            full = p[name].transpose(1, 2).contiguous()
+            full[page, off] = (x * inv.double()[..., None]).float().round().to(full.dtype)
+            res.append(full.transpose(1, 2))
         else:
             full = p[name].double().transpose(1, 2).contiguous()
             full[page, off] = x
