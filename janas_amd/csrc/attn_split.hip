@@ -365,11 +365,7 @@ __global__ __launch_bounds__(kSW * 64) __attribute__((amdgpu_waves_per_eu(D <= 1
             }
             continue;
         }
-        int ex = 0;
-        if (mx > 0.0f && mx < INFINITY) {
-            frexpf(mx, &ex);
-            ex = 14 - ex;
-        }
+        const int ex = query_exponent(mx);
         const float up = ldexpf(1.0f, ex);
         if (qrow[h] < kTileRows) {
 #pragma unroll

@@ -253,11 +253,7 @@ __global__ __launch_bounds__(256) void wide_kernel(const SplitArgs A)
             if (l16 == 0)
                 sQs[qrow] = mx / 32767.0f;
         } else {
-            int ex = 0;
-            if (mx > 0.0f && mx < INFINITY) {
-                frexpf(mx, &ex);
-                ex = 14 - ex;
-            }
+            const int ex = query_exponent(mx);
             const float up = ldexpf(1.0f, ex);
 #pragma unroll
             for (int i = 0; i < S::QV; i++) {
