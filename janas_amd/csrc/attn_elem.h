@@ -226,11 +226,11 @@ __device__ __forceinline__ uint32_t scan_wave(uint32_t x)
     return x;
 }
 
-/* The power of two that puts a query row's largest number, mx, in [2^13, 2^14)
-   before it is split into planes. At most 2^126, so that it and its reciprocal
-   are numbers: a row below 2^-113 then loses bits of 2^-150 and less, which no
-   score shows unless keys pass 2^100 */
-__device__ __forceinline__ int query_exponent(float mx)
+/* The power of two that puts the largest number, mx, of what is split into planes
+   (a query row; a wave's value scales) in [2^13, 2^14). At most 2^126, so that it and its reciprocal
+   are numbers: a query row below 2^-113 then loses bits of 2^-150 and less, which
+   no score shows unless keys pass 2^100 */
+__device__ __forceinline__ int plane_exponent(float mx)
 {
     int ex;
     frexpf(fmaxf(mx, 0x1p-113f), &ex);

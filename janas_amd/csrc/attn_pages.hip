@@ -543,7 +543,7 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
                 *(f4 *)&sQ[qrow][qc[j]] = qx[j];
         } else {
             qmax = max_x16(max_row16(qmax)); /* the row's 32 lanes */
-            const int ex = query_exponent(qmax);
+            const int ex = plane_exponent(qmax);
             const float up = ldexpf(1.0f, ex), neg1 = minus_one();
 #pragma unroll
             for (int j = 0; j < NQ; j++) {

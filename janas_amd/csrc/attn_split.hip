@@ -365,7 +365,7 @@ __global__ __launch_bounds__(kSW * 64) __attribute__((amdgpu_waves_per_eu(D <= 1
             }
             continue;
         }
-        const int ex = query_exponent(mx);
+        const int ex = plane_exponent(mx);
         const float up = ldexpf(1.0f, ex);
         if (qrow[h] < kTileRows) {
 #pragma unroll
@@ -690,10 +690,7 @@ __global__ __launch_bounds__(kSW * 64) __attribute__((amdgpu_waves_per_eu(D <= 1
         for (int s = 0; s < kSNG; s++)
             vm = fmaxf(vm, fmaxf(vz2[s].x, vz2[s].y));
         vm = max_x32(max_x16(fmaxf(vm, from_x1(vm))));
-        int ev = 0;
-        if (vm > 0.0f && vm < INFINITY)
-            frexpf(vm, &ev);
-        pe = 13 - ev;
+        pe = plane_exponent(vm) - 1;
     }
     if constexpr (!Q16) {
         const float up = ldexpf(1.0f, pe);

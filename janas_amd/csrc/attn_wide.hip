@@ -253,7 +253,7 @@ __global__ __launch_bounds__(256) void wide_kernel(const SplitArgs A)
             if (l16 == 0)
                 sQs[qrow] = mx / 32767.0f;
         } else {
-            const int ex = query_exponent(mx);
+            const int ex = plane_exponent(mx);
             const float up = ldexpf(1.0f, ex);
 #pragma unroll
             for (int i = 0; i < S::QV; i++) {
@@ -471,10 +471,7 @@ __global__ __launch_bounds__(256) void wide_kernel(const SplitArgs A)
                 for (int e = 0; e < 4 * kRounds; e++)
                     vm = fmaxf(vm, vsc[e]);
                 vm = max_x32(max_x16(vm));
-                int ev = 0;
-                if (vm > 0.0f && vm < INFINITY)
-                    frexpf(vm, &ev);
-                pe = 13 - ev;
+                pe = plane_exponent(vm) - 1;
             }
             const float up = ldexpf(1.0f, pe);
 #pragma unroll

@@ -1,8 +1,8 @@
-"""Query rows far below one, down to subnormal numbers, beside ordinary rows and
-rows of zeros: the planes' power of two stays a number. Every kernel that takes
-the query as planes, over every cache type, at head sizes that fill their tiles
-and that do not. All scores are then next to 0 and a row is the mean of the
-values in sight."""
+"""Query rows and value scales far below one: the planes' power of two stays a
+number. Query rows down to subnormal numbers, beside ordinary rows and rows of
+zeros; every kernel that takes the query as planes, over every cache type, at
+head sizes that fill their tiles and that do not. All scores are then next to 0
+and a row is the mean of the values in sight."""
 import numpy as np
 import pytest
 import torch
@@ -64,29 +64,47 @@ def test_pages(gpu, kv, hd):
     check(pool, q[:, None], out.cpu().numpy()[:, None], f"pages {NAMES[kv]} {hd}")
 
 
+def run_contiguous(gpu, pool, q, kv, cap=1100):
+    """The split kernels (head sizes to 256, and above) over the pool's one
+    sequence of 1000 rows, the last of q's tokens at its end."""
+    dev = lambda x: torch.from_numpy(x).to(gpu)  # noqa: E731
+    rows, p = {}, np.arange(1000)
+    for name, x in (("k", pool.k), ("v", pool.v), ("ks", pool.ks), ("vs", pool.vs)):
+        if x is None:
+            continue
+        y = np.zeros((pool.n_kv, cap) + x.shape[3:], x.dtype)
+        y[:, :1000] = np.moveaxis(x[pool.table[0, p // 256], :, p % 256], 0, 1)
+        rows[name] = dev(y)
+    n, h = q.shape[:2]
+    out = torch.zeros(q.shape, device=gpu)
+    with jm.Attention(h, pool.n_kv, pool.hd, cap, 1, jm.FLOAT) as a:
+        a.run_dev(kv, [dict(rows, q=dev(q), out=out, cap=cap, n=n, pos0=1000 - n)], path="split")
+        torch.cuda.synchronize()
+    return out.cpu().numpy()
+
+
 # (f32 rows above 128 are refused)
 @pytest.mark.parametrize("n", [1, 3])
 @pytest.mark.parametrize("kv,hd", [(kv, hd) for kv, hd in CASES if kv != KV_F32 or hd <= 128],
                          ids=lambda x: str(x))
 def test_contiguous(gpu, kv, hd, n):
-    """The split kernels (head sizes to 256, and above)."""
-    h, n_kv, cap = 10, 1, 1100
+    h = 10
     rng = np.random.default_rng([kv, hd, n])
-    pool = ph.Pool(rng, kv, [1000], 256, n_kv, hd)
-    pool.table = pool.table[:, :4]
-    q = queries(rng, n, h, hd)[None]
-    dev = lambda x: None if x is None else torch.from_numpy(x).to(gpu)  # noqa: E731
-    rows = {}
-    for name, x in (("k", pool.k), ("v", pool.v), ("ks", pool.ks), ("vs", pool.vs)):
-        if x is None:
-            continue
-        y = np.zeros((n_kv, cap) + x.shape[3:], x.dtype)
-        p = np.arange(1000)
-        y[:, :1000] = np.moveaxis(x[pool.table[0, p // 256], :, p % 256], 0, 1)
-        rows[name] = dev(y)
-    out = torch.zeros(q.shape[1:], device=gpu)
-    with jm.Attention(h, n_kv, hd, cap, 1, jm.FLOAT) as a:
-        a.run_dev(kv, [dict(rows, q=dev(q[0]), out=out, cap=cap, n=n, pos0=1000 - n)], path="split")
-        torch.cuda.synchronize()
-    check(pool, q, out.cpu().numpy()[None], f"split {NAMES[kv]} {hd}",
+    pool = ph.Pool(rng, kv, [1000], 256, 1, hd)
+    q = queries(rng, n, h, hd)
+    check(pool, q[None], run_contiguous(gpu, pool, q, kv)[None], f"split {NAMES[kv]} {hd}",
           seen=lambda m, t: m - n + t + 1)
+
+
+@pytest.mark.parametrize("down", [100, 108, 110, 112])
+@pytest.mark.parametrize("kv,hd", [(kv, hd) for kv, hd in CASES if kv in ph.TOP],
+                         ids=lambda x: str(x))
+def test_contiguous_value_scales(gpu, kv, hd, down):
+    """Scales of N(0, 1) rows times 2^-down: on both sides of 2^-115 (int8, 2^-5
+    of a number; int16 2^-13), all numbers normal floats."""
+    down -= 8 if kv == KV_I16 else 0
+    rng = np.random.default_rng([kv, hd, down])
+    pool = ph.Pool(rng, kv, [1000], 256, 1, hd)
+    pool.vs *= np.float32(2.0 ** -down)
+    q = rng.standard_normal((1, 10, hd)).astype(np.float32)
+    check(pool, q[None], run_contiguous(gpu, pool, q, kv)[None], f"scales {NAMES[kv]} {hd}")
