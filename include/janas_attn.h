@@ -520,8 +520,9 @@ size_t janas_attn_pages_work_bytes(const struct janas_attn *a,
  * counts twice). A row that sees nothing is 0. The instance gives heads,
  * scale and window; its scores are FLOAT's whatever its way, float-accurate
  * over every cache type: within 1e-5 of softmax-normalized outputs. A page
- * outside the pool, or a length past the table row, makes the row NaN;
- * nothing outside the arrays is read. What is cached out of sight counts for
+ * outside the pool of a block in sight, or a length past the table row, makes
+ * the row NaN (the table entries of blocks before the window are not used,
+ * listed or not); nothing outside the arrays is read. What is cached out of sight counts for
  * nothing, NaN and infinities included; an infinite number in sight may make
  * a row NaN. How a sequence's positions are split depends on all the lengths
  * of the call, so a row's last bits may differ from one batch to another (the

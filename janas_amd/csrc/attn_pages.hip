@@ -399,7 +399,9 @@ __attribute__((amdgpu_waves_per_eu(PS<T, D>::WAVES))) void pages_kernel(const Pa
             const uint32_t lim = ((last > first ? last : su + u0) - 1) >> upp_log;
             const uint32_t e = from + lane < lim ? from + lane : lim;
             blk = SEL ? srow[e] : e;
-            const bool in = blk < nb;
+            /* (a listed block before the window, whose page may be gone, counts
+               for as little as one past the end) */
+            const bool in = blk < nb && (!SEL || blk >= sv.lo >> A.page_log);
             pid = trow[in ? blk : 0];
             bad |= in && pid >= A.n_pages;
             pid = in && pid < A.n_pages ? pid : 0;

@@ -523,6 +523,43 @@ def test_run_selected(gpu, kv, window):
     assert not out[4, :h // n_kv].any() and not out[2].any()
 
 
+@pytest.mark.parametrize("kv", [KV_I8, KV_I16, KV_F16, KV_F32], ids=NAMES.get)
+@pytest.mark.parametrize("window", [1, 16, 77, 150])
+def test_run_selected_blocks_before_the_window(gpu, kv, window):
+    """A list kept for some steps while the window goes on: the pages of the
+    blocks that it has left may be gone, and their table entries anything. A
+    block that the window begins in is still read, and is bad if its page is."""
+    h, n_kv, hd, page = 8, 2, 64, 32
+    rng = np.random.default_rng([kv, window])
+    lens = [500, 33, 0, 1025, 320, 700, 64]
+    pool = ph.Pool(rng, kv, lens, page, n_kv, hd)
+    n_sel = 9
+    sel = np.full((len(lens), n_kv, n_sel), ph.NONE, np.int32)
+    for i, n in enumerate(lens):
+        nb = ph.blocks(n, page)
+        for kh in range(n_kv):
+            m = min(nb, n_sel)
+            sel[i, kh, :m] = rng.permutation(nb)[:m]
+            sel[i, kh, :min(m, 2)] = [nb - 1, 0][:min(m, 2)]
+    q = rng.standard_normal((len(lens), h, hd)).astype(np.float32)
+    whole = pool.table.copy()
+    for i, n in enumerate(lens):
+        for b in range(max(0, n - window) // page):
+            pool.table[i, b] = (0x7FFFFF00, -1, pool.n_pages)[b % 3]
+    gone = pool.table.copy()
+    out = run_pages(gpu, pool, h, q, window=window, sel=sel, times=2)
+    pool.table = whole
+    check_run(pool, h, q, out, window=window, sel=sel, what="blocks before the window")
+    # the first block in sight of the longest sequence, gone too
+    b = (1025 - window) // page
+    pool.table = gone
+    pool.table[3, b] = -1
+    sel[3, 0, 1] = b
+    bad = run_pages(gpu, pool, h, q, window=window, sel=sel)
+    assert np.isnan(bad[3, :h // n_kv]).all()
+    assert np.array_equal(bad[[0, 1, 2, 4, 5, 6]], out[[0, 1, 2, 4, 5, 6]])
+
+
 # ---- bounds and selection ---------------------------------------------------
 
 @pytest.mark.parametrize("kv", [KV_I8, KV_I16, KV_F16, KV_F32], ids=NAMES.get)
