@@ -507,8 +507,14 @@ struct janas_attn_pages_call {
                                 (n_rows of them with row, else n_seqs) */
 };
 
-/* Device bytes that a janas_attn_pages_run or _select over p needs as work;
-   0 where the call would be refused. */
+/* Device bytes that a janas_attn_pages_run over p needs as work and, where p has
+   bounds, a _select (ask with them set if it will be called); 0 where either
+   call is refused whatever it is given. They follow from p's sizes, the
+   instance's heads and the device. The run refuses n_seqs x max_pages x page of
+   2^35 positions and more, the selection max_pages above 2^20, and both what a
+   launch cannot hold: 2^24 workgroups of 256 threads (n_seqs x n_head x
+   ceil(head_dim / 32) below that always fits), 2^22 (sequence, KV head) pairs
+   of a selection. */
 size_t janas_attn_pages_work_bytes(const struct janas_attn *a,
                                    const struct janas_attn_pages *p);
 

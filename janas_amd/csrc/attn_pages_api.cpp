@@ -106,7 +106,7 @@ int check_rows(const PagesGeom &g, const janas_attn_pages_call *c)
         (c->q_stride && c->q_stride < width) || !c->row != !c->granted ||
         !aligned(c->work, 256))
         return JANAS_ATTN_EINVAL;
-    return width > 0xFFFFFFFFu ? JANAS_ATTN_ERANGE : JANAS_ATTN_OK;
+    return JANAS_ATTN_OK;
 }
 
 /* no rows, so that no sequence takes part */
@@ -138,6 +138,30 @@ Parts parts_of(const PagesGeom &g, const janas_attn_pages *p)
 uint64_t score_bytes(const janas_attn_pages *p)
 {
     return (uint64_t)p->n_seqs * p->n_kv * p->max_pages * sizeof(float);
+}
+
+/* whether the pool's and the instance's sizes alone let janas_attn_pages_run ... */
+int run_fits(const PagesGeom &g, const janas_attn_pages *p, const Parts &t)
+{
+    if ((uint64_t)g.n_head * g.hd > 0xFFFFFFFFu || g.n_head > 65535)
+        return JANAS_ATTN_ERANGE;
+    /* a call's units of 16 positions (and what rounds them up) in 32 bits */
+    if ((uint64_t)p->n_seqs * p->max_pages * (p->page / 16) >= 1ull << 31)
+        return JANAS_ATTN_ERANGE;
+    const uint64_t cols = pages_merge_cols(p->n_seqs, g.n_head, g.hd);
+    const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + cols - 1) / cols);
+    return std::max((t.runs + 1) * g.n_kv * t.rtiles, merge_wg) > kMostThreads / 256
+               ? JANAS_ATTN_ERANGE
+               : JANAS_ATTN_OK;
+}
+
+/* ... and janas_attn_pages_select take them */
+int select_fits(const PagesGeom &g, const janas_attn_pages *p)
+{
+    return (uint64_t)g.n_head * g.hd > 0xFFFFFFFFu || p->max_pages > 1u << 20 ||
+                   (uint64_t)p->n_seqs * p->n_kv > kMostThreads / 1024
+               ? JANAS_ATTN_ERANGE
+               : JANAS_ATTN_OK;
 }
 
 }  // namespace
@@ -280,8 +304,11 @@ extern "C" size_t janas_attn_pages_work_bytes(const struct janas_attn *a,
 {
     if (check_instance(a, p))
         return 0;
-    const uint64_t run = parts_of(pages_geom(a), p).bytes;
-    return (size_t)(p->bounds ? std::max(run, score_bytes(p)) : run);
+    const PagesGeom g = pages_geom(a);
+    const Parts t = parts_of(g, p);
+    if (run_fits(g, p, t) || (p->bounds && select_fits(g, p)))
+        return 0;
+    return (size_t)(p->bounds ? std::max(t.bytes, score_bytes(p)) : t.bytes);
 }
 
 extern "C" int janas_attn_pages_run(struct janas_attn *a,
@@ -305,17 +332,12 @@ extern "C" int janas_attn_pages_run(struct janas_attn *a,
         (c->out_q8k && (uint64_t)g.n_head * g.hd % JANAS_ATTN_QK))
         return JANAS_ATTN_EINVAL;
     const Parts t = parts_of(g, p);
-    /* a call's units of 16 positions (and what rounds them up) in 32 bits */
-    if ((uint64_t)p->n_seqs * p->max_pages * (p->page / 16) >= 1ull << 31)
-        return JANAS_ATTN_ERANGE;
-    const uint64_t cols = pages_merge_cols(p->n_seqs, g.n_head, g.hd);
-    const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + cols - 1) / cols);
+    rc = run_fits(g, p, t);
+    if (rc)
+        return rc;
     const uint64_t rows = c->row ? c->n_rows : p->n_seqs;
     const uint64_t blocks = rows * g.n_head * g.hd / JANAS_ATTN_QK;
-    if (std::max({(t.runs + 1) * g.n_kv * t.rtiles, merge_wg, c->out_q8k ? blocks : 0}) >
-            kMostThreads / 256 || g.n_head > 65535)
-        return JANAS_ATTN_ERANGE;
-    if (c->work_bytes < t.bytes)
+    if ((c->out_q8k && blocks > kMostThreads / 256) || c->work_bytes < t.bytes)
         return JANAS_ATTN_ERANGE;
     PagesArgs s;
     memset(&s, 0, sizeof s);
@@ -384,8 +406,10 @@ extern "C" int janas_attn_pages_select(struct janas_attn *a,
         return rc;
     if (!p->bounds || !sel || !c->work || c->n_sel == 0 || (uint64_t)first + last > c->n_sel)
         return JANAS_ATTN_EINVAL;
-    if (p->max_pages > 1u << 20 || (uint64_t)p->n_seqs * p->n_kv > kMostThreads / 1024 ||
-        c->work_bytes < score_bytes(p))
+    rc = select_fits(g, p);
+    if (rc)
+        return rc;
+    if (c->work_bytes < score_bytes(p))
         return JANAS_ATTN_ERANGE;
     SelectArgs s;
     memset(&s, 0, sizeof s);
