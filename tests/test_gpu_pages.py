@@ -230,6 +230,53 @@ def test_write_is_the_contiguous_write(gpu, kv, case, how):
     assert bool((pks.transpose(1, 2)[kept] == 7.5).all())
 
 
+@pytest.mark.parametrize("kv", [KV_I8, KV_I16, KV_F16, KV_F32], ids=NAMES.get)
+@pytest.mark.parametrize("hd,n_rot", [(128, 128), (128, 0), (40, 36)])
+@pytest.mark.parametrize("how", ["in place", "apart", "no queries"])
+def test_write_leaves_rows_out(gpu, kv, hd, n_rot, how):
+    """Rows without a slot, with one outside the pool, or at a position that the
+    table does not have: nothing of them is written, their queries neither, which
+    in place are the caller's own; the other rows are those of a call without
+    them."""
+    n, h, n_kv, page, n_pages, n_tab = 9, 4, 2, 16, 3, 50
+    rng = np.random.default_rng([kv, hd, n_rot])
+    cs, sn = (dev(x, gpu) for x in ph.rotation(n_tab, n_rot))
+    x = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).to(gpu)  # noqa: E731
+    q, k, v, kn, qn = x(n, h, hd), x(n, n_kv, hd), x(n, n_kv, hd), x(hd), x(hd)
+    slot = torch.from_numpy(rng.permutation(n_pages * page)[:n].astype(np.int32)).to(gpu)
+    pos = torch.arange(n, dtype=torch.int32, device=gpu)
+    slot[1], slot[4], slot[8] = ph.NONE, n_pages * page, 0x7FFFFFFF
+    left = [1, 4, 8]
+    if n_rot:
+        pos[5], pos[6] = n_tab, -1
+        left += [5, 6]
+    kept = [t for t in range(n) if t not in left]
+    dt = {KV_I8: torch.int8, KV_I16: torch.int16, KV_F16: torch.float16, KV_F32: torch.float32}[kv]
+    table = torch.zeros(1, 1, dtype=torch.int32, device=gpu)
+
+    def written(rows):
+        pool = [torch.full((n_pages, n_kv, page, hd), 77, dtype=dt, device=gpu) for _ in range(2)]
+        pool += [torch.full((n_pages, n_kv, page), 7.5, device=gpu) for _ in range(2)]
+        p = at.pages(*pool, kv_type=kv, table=table, length=table[0])
+        qq = q[rows].clone()
+        out = qq if how == "in place" else torch.full_like(qq, 3.25)
+        more = {} if how == "no queries" else dict(q=qq, q_out=out, q_norm=qn)
+        at.pages_write(p, k[rows].clone(), v[rows].clone(), slot=slot[rows].clone(),
+                       pos=pos[rows].clone(), cs=cs, sn=sn, n_rot=n_rot, k_norm=kn, **more)
+        torch.cuda.synchronize()
+        return pool, out
+    (pool, out), (pool2, out2) = written(list(range(n))), written(kept)
+    for y, z in zip(pool, pool2):
+        assert torch.equal(y, z)
+    assert torch.equal(out[kept], out2)
+    before = q if how == "in place" else torch.full_like(q, 3.25)
+    assert torch.equal(out[left], before[left])
+    if how == "no queries":
+        assert bool((out == 3.25).all())
+    else:
+        assert not bool((out[kept] == before[kept]).flatten(1).all(1).any())
+
+
 # ---- attention --------------------------------------------------------------
 
 def run_pages(gpu, pool, h, q, *, window=0, gate=None, mode=jm.GATE_NONE, sel=None, scale=None,
