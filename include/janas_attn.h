@@ -479,7 +479,8 @@ int janas_attn_pages_write(const struct janas_attn_pages *p,
  * rounded outward and kept within +-65504 (NaN keys are passed over; a block
  * of nothing else gets 65504, -65504). A page that several sequences share gets
  * those of one of them: the same ones where it is full. max_new: the largest
- * n_new, for the launch's size only (0: not known).
+ * n_new, for the launch's size only (0: not known). JANAS_ATTN_ERANGE: n_seqs x
+ * n_kv x ceil(head_dim / 128) of 2^24 and more.
  */
 int janas_attn_pages_bounds(const struct janas_attn_pages *p,
                             const uint32_t *n_new, uint32_t max_new,

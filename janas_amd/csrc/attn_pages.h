@@ -99,6 +99,12 @@ struct BoundsArgs {
     uint32_t n_seqs, n_kv, hd, max_pages, n_pages, page_log, max_blocks;
     int kv;
 };
+/* columns a workgroup takes, and with that the workgroups a block and KV head */
+constexpr uint32_t kBoundCols = 128;
+__host__ __device__ constexpr uint32_t bound_slices(uint32_t hd)
+{
+    return (hd + kBoundCols - 1) / kBoundCols;
+}
 hipError_t launch_bounds(const BoundsArgs &a, hipStream_t s);
 struct SelectArgs {
     const _Float16 *bounds;

@@ -285,11 +285,12 @@ extern "C" int janas_attn_pages_bounds(const struct janas_attn_pages *p,
     a.n_pages = p->n_pages;
     a.page_log = log2_of(p->page);
     a.kv = p->kv_type;
-    /* a workgroup each at least */
-    if ((uint64_t)p->n_seqs * p->n_kv > kMostThreads / 256)
+    /* a workgroup of each at least, for every 128 columns */
+    if ((uint64_t)p->n_seqs * p->n_kv * bound_slices(a.hd) > kMostThreads / 256)
         return JANAS_ATTN_ERANGE;
     /* the blocks that max_new positions may touch; a workgroup goes on to
-       further ones */
+       further ones (2^20 x 4 workgroups or one a block's slice: a launch holds
+       them) */
     uint64_t blocks = p->max_pages;
     if (n_new && max_new)
         blocks = std::min<uint64_t>(blocks, ((uint64_t)max_new + p->page - 2) / p->page + 1);

@@ -71,11 +71,6 @@ template <int KV> __device__ __forceinline__ typename Raw8<KV>::T load8(const vo
 }
 
 constexpr uint32_t kBoundRows = 4;     /* rows a thread asks for at once */
-constexpr uint32_t kBoundCols = 128;   /* columns a workgroup takes */
-__host__ __device__ constexpr uint32_t bound_slices(uint32_t hd)
-{
-    return (hd + kBoundCols - 1) / kBoundCols;
-}
 
 /*
  * A workgroup takes up to 128 columns of one block and KV head: its threads take 8

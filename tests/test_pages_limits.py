@@ -37,6 +37,7 @@ def calls(tmp_path_factory):
                                        ctypes.POINTER(at.PagesCall), vp]
     L.janas_attn_pages_select.argtypes = [vp, ctypes.POINTER(at.Pages),
                                           ctypes.POINTER(at.PagesCall), u32, u32, vp, vp]
+    L.janas_attn_pages_bounds.argtypes = [ctypes.POINTER(at.Pages), vp, u32, vp]
     return L
 
 
@@ -98,3 +99,14 @@ def test_work_bytes_and_the_calls_agree(calls):
         assert (size == 0) == refused, (size, run, sel, [(x, getattr(p, x)) for x, _ in p._fields_])
         both[0 if not refused else 1 if run else 2] += 1
     assert min(both) > 100, both
+
+
+@pytest.mark.parametrize("n_seqs,n_kv,hd,code", [
+    (65535, 256, 128, jm.OK), (65535, 257, 128, jm.ERANGE), (65535, 128, 136, jm.OK),
+    (65535, 129, 136, jm.ERANGE), (65535, 64, 512, jm.OK), (65535, 65, 512, jm.ERANGE),
+    (1, 65535, 512, jm.OK)])
+def test_bounds_take_what_a_launch_holds(calls, n_seqs, n_kv, hd, code):
+    """Below 2^24 workgroups of 256 threads, one for every 128 columns."""
+    p, before = pool(n_seqs=n_seqs, n_kv=n_kv, head_dim=hd), calls.launched()
+    assert calls.janas_attn_pages_bounds(ctypes.byref(p), A, 1, None) == code
+    assert calls.launched() - before == (code == jm.OK)
