@@ -436,8 +436,10 @@ struct janas_attn_plan {
  * row (max_pages x page) or the packed rows (max_tokens), and, from the first
  * one that finds too few free pages on, every sequence that needs one (those
  * that need none go on). A page that two released rows name is returned twice;
- * that, and table entries outside the pool, are not checked here; no write leaves
- * the arrays. n_free above n_pages counts as n_pages.
+ * that is not checked here. Nor are table entries and free pages outside the
+ * pool: they go where pages go, but a token of theirs has no slot
+ * (JANAS_ATTN_NONE). No write leaves the arrays. n_free above n_pages counts as
+ * n_pages.
  */
 int janas_attn_pages_plan(const struct janas_attn_pages *p,
                           const struct janas_attn_plan *s, void *stream);

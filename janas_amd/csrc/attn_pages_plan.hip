@@ -62,6 +62,13 @@ __device__ __forceinline__ uint32_t stack_page(const PlanArgs &A, uint64_t top, 
     return k < top ? A.free_pages[top - 1 - k] : 0;
 }
 
+/* position p's slot in its page; none where the table or the stack names a page
+   outside the pool, whose slots in 32 bits could be another page's */
+__device__ __forceinline__ uint32_t slot_of(const PlanArgs &A, uint32_t page, uint32_t p)
+{
+    return page < A.n_pages ? (page << A.page_log) + (p & ((1u << A.page_log) - 1)) : kNone;
+}
+
 /* the last i of n with at[i] <= x (at[0] = 0) */
 __device__ __forceinline__ uint32_t last_at(const uint32_t *at, uint32_t n, uint32_t x)
 {
@@ -174,9 +181,9 @@ __global__ __launch_bounds__(WAVES * 64) void plan_kernel(const PlanArgs A)
             if (ok && need)
                 row[have] = page;
             if (add && first < A.max_tokens) {
-                const uint32_t in = old & ((1u << A.page_log) - 1);
-                A.slot[first] = ok ? (page << A.page_log) + in : kNone;
-                A.pos[first] = ok ? old : 0;
+                const uint32_t s = ok ? slot_of(A, page, old) : kNone;
+                A.slot[first] = s;
+                A.pos[first] = s != kNone ? old : 0;
                 A.seq[first] = i;
             }
         }
@@ -207,10 +214,10 @@ __global__ __launch_bounds__(WAVES * 64) void plan_kernel(const PlanArgs A)
                         p = o + t;
                         const uint32_t b = p >> A.page_log;
                         s = b < h ? row[b] : stack_page(A, top, sTake[k] + b - h);
-                        s = (s << A.page_log) + (p & ((1u << A.page_log) - 1));
+                        s = slot_of(A, s, p);
                     }
                     A.slot[at + t] = s;
-                    A.pos[at + t] = p;
+                    A.pos[at + t] = s != kNone ? p : 0;
                     A.seq[at + t] = i0 + k;
                 }
             }
@@ -274,11 +281,11 @@ __global__ __launch_bounds__(256) void plan_fill_kernel(const PlanArgs A, uint32
             const uint32_t b = p >> A.page_log;
             s = b < h ? A.table[(size_t)i * A.max_pages + b]
                       : stack_page(A, top, (uint64_t)take + b - h);
-            s = (s << A.page_log) + (p & ((1u << A.page_log) - 1));
+            s = slot_of(A, s, p);
         }
     }
     A.slot[t] = s;
-    A.pos[t] = p;
+    A.pos[t] = s != kNone ? p : 0;
     A.seq[t] = i;
 }
 

@@ -144,6 +144,38 @@ def test_plan_bad_counts_stay_in_the_arrays(gpu):
     assert canaries_whole(wt, wf, *whole.values())
 
 
+@pytest.mark.parametrize("tokens", [1, 3, 70])
+@pytest.mark.parametrize("rows", [100, 5000])
+def test_plan_pages_outside_the_pool_have_no_slots(gpu, tokens, rows):
+    """Pages whose slots would be another's in 32 bits (2^28 pages of 16 are 2^32
+    slots), named by the table or on the stack: the tokens that would lie there
+    have none, the others theirs. In one launch and in two."""
+    page, n_pages = 16, 12
+    wild = 1 << 28
+    table = torch.tensor([[wild, 1, 0, 0, 0, 0], [2, wild + 1, 0, 0, 0, 0], [3, 0, 0, 0, 0, 0],
+                          [4, 5, 0, 0, 0, 0]], dtype=torch.int32, device=gpu)
+    lens = [7, 20, 16, 17]
+    free = torch.zeros(n_pages, dtype=torch.int32, device=gpu)
+    # (from the top: the third page that the step takes is outside)
+    free[:6] = torch.tensor([9, 8, 7, wild + 2, 6, 10], dtype=torch.int32)
+    out = {name: torch.full((m,), CANARY, dtype=torch.int32, device=gpu)
+           for name, m in dict(length=4, n_free=1, granted=4, start=5, taken=5, slot=rows, pos=rows,
+                               seq=rows).items()}
+    n_new = [tokens if tokens < 70 else x for x in (20, 3, 30, 0)]
+    p = at.page_tables(table, dev(np.array(lens, np.int32), gpu), page=page, free=free,
+                       n_free=torch.full((1,), 6, dtype=torch.int32, device=gpu))
+    at.pages_plan(p, dev(np.array(n_new, np.int32), gpu), **out)
+    torch.cuda.synchronize()
+    assert out["granted"].tolist() == n_new
+    at_ = [(pos, int(table[i, pos // page])) for i, n in enumerate(n_new)
+           for pos in range(lens[i], lens[i] + n)]
+    want = [pg * page + pos % page if pg < n_pages else -1 for pos, pg in at_]
+    behind = rows - len(want)
+    assert out["slot"].tolist() == want + [-1] * behind
+    assert out["pos"].tolist() == [pos if pg < n_pages else 0 for pos, pg in at_] + [0] * behind
+    assert -1 in want and max(want) >= 0
+
+
 # ---- write ------------------------------------------------------------------
 
 # tokens, query heads, KV heads, hd, n_rot, norms, v_norm, page
