@@ -505,6 +505,8 @@ def _rows_of(x, what, shape):
         return 0
     if x.stride(0) < shape[1] * shape[2]:
         raise ValueError(f"{what}'s rows overlap")
+    if x.stride(0) > 0xFFFFFFFF:
+        raise ValueError(f"{what}'s rows are {x.stride(0)} floats apart, more than 32 bits hold")
     return x.stride(0)
 
 

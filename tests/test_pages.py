@@ -161,6 +161,24 @@ def test_python_refuses_other_devices():
                                          length=t["length"]))
 
 
+def test_python_refuses_strides_past_32_bits():
+    """The structures hold them in 32 bits: 2^32 + 128 would be 128."""
+    import torch
+    far = lambda n: torch.empty_strided((2, n, 64), ((1 << 32) + 64 * n, 64, 1),  # noqa: E731
+                                        device="meta")
+    near = lambda n: torch.empty(2, n, 64, device="meta")  # noqa: E731
+    k = torch.empty(8, 2, 16, 64, dtype=torch.float16, device="meta")
+    slot = torch.empty(2, dtype=torch.int32, device="meta")
+    t = dict(table=torch.empty(2, 4, dtype=torch.int32, device="meta"),
+             length=torch.empty(2, dtype=torch.int32, device="meta"))
+    p = at.pages(k, k, kv_type=jm.KV_F16, **t)
+    at.prepare_pages_write(p, near(2), near(2), slot=slot, q=near(4))
+    for x in (dict(k=far(2)), dict(v=far(2)), dict(q=far(4), q_out=near(4))):
+        x = dict(dict(k=near(2), v=near(2), q=near(4)), **x)
+        with pytest.raises(ValueError, match="32 bits"):
+            at.prepare_pages_write(p, x.pop("k"), x.pop("v"), slot=slot, **x)
+
+
 def test_plain_plan_keeps_pages_apart():
     """The restatement itself: over random steps every page is in one place -
     the free ones or one table row - and none is lost."""
