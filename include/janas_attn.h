@@ -514,7 +514,7 @@ struct janas_attn_pages_call {
    bounds, a _select (ask with them set if it will be called); 0 where either
    call is refused whatever it is given. They follow from p's sizes, the
    instance's heads and the device. The run refuses n_seqs x max_pages x page of
-   2^35 positions and more, the selection max_pages above 2^20, and both what a
+   2^34 positions and more, the selection max_pages above 2^20, and both what a
    launch cannot hold: 2^24 workgroups of 256 threads (n_seqs x n_head x
    ceil(head_dim / 32) below that always fits), 2^22 (sequence, KV head) pairs
    of a selection. */

@@ -145,8 +145,9 @@ int run_fits(const PagesGeom &g, const janas_attn_pages *p, const Parts &t)
 {
     if ((uint64_t)g.n_head * g.hd > 0xFFFFFFFFu || g.n_head > 65535)
         return JANAS_ATTN_ERANGE;
-    /* a call's units of 16 positions (and what rounds them up) in 32 bits */
-    if ((uint64_t)p->n_seqs * p->max_pages * (p->page / 16) >= 1ull << 31)
+    /* a call's units of 16 positions in 32 bits, with what rounds them up and times
+       the four waves that share them */
+    if ((uint64_t)p->n_seqs * p->max_pages * (p->page / 16) >= 1ull << 30)
         return JANAS_ATTN_ERANGE;
     const uint64_t cols = pages_merge_cols(p->n_seqs, g.n_head, g.hd);
     const uint64_t merge_wg = (uint64_t)p->n_seqs * g.n_head * ((g.hd + cols - 1) / cols);

@@ -62,10 +62,12 @@ def answers(L, h, p, ring=0, work=MOST):
 
 @pytest.mark.parametrize("over,run,sel", [
     (dict(), jm.OK, jm.OK),
-    # 2^31 units of 16 positions, and one table row fewer
-    (dict(n_seqs=1 << 11, max_pages=1 << 20), jm.ERANGE, jm.OK),
-    (dict(n_seqs=(1 << 11) - 1, max_pages=1 << 20), jm.OK, jm.OK),
-    (dict(n_seqs=1 << 8, max_pages=1 << 20, page=128), jm.ERANGE, jm.OK),
+    # 2^30 units of 16 positions, and one table row fewer: a workgroup may have
+    # them all, and a wave's share of them is (units x 3) / 4 and (units x 4) / 4
+    # in 32 bits
+    (dict(n_seqs=1 << 10, max_pages=1 << 20), jm.ERANGE, jm.OK),
+    (dict(n_seqs=(1 << 10) - 1, max_pages=1 << 20), jm.OK, jm.OK),
+    (dict(n_seqs=1 << 7, max_pages=1 << 20, page=128), jm.ERANGE, jm.OK),
     # more blocks than a selection takes
     (dict(max_pages=(1 << 20) + 1), jm.OK, jm.ERANGE),
     # more workgroups than a launch takes: the merge's, the selection's
