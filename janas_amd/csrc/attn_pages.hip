@@ -92,14 +92,17 @@ constexpr uint32_t kLeastUnits = kPW;
  * rounded up to whole runs), so that no workgroup has two.
  *
  * Every wave finds its part for itself, a lane a sequence, 64 at a time; what it
- * will want of them stays in LDS.
+ * will want of them stays in LDS. Up to 64 sequences that is one load; above, three
+ * passes over them at most, some 18 us a thousand (one sequence of 1000 positions
+ * beside empty ones: 5.2 us up to 64, 7.6 of 256, 18.5 of 1024, 72 of 4096).
  */
 struct RunsLds {
     uint32_t row[64], lo[64], end[64], units[64];
     uint32_t from[64], to[64];   /* a sequence's units in the launch's */
 };
 
-/* (units count in 32 bits: janas_attn_pages_run refuses tables that hold more) */
+/* (units count in 32 bits, four times as many too: janas_attn_pages_run refuses
+   tables that hold more) */
 template <bool SEL> struct Runs {
     uint32_t i0, per, whole;     /* units a run; each sequence in whole runs */
     uint32_t runs;               /* of the launch */
